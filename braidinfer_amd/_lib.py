@@ -24,6 +24,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libbraidinfer_amd.so"
 ABI_VERSION = 1
 
 F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
+FP4 = 5  # BFA_DTYPE_FP4: the 4-bit cache
 DTYPE_CODE = _DTYPE_CODE = {
     torch.float32: F32,
     torch.float16: F16,
@@ -115,6 +116,23 @@ _SIGNATURES = {
     "bfa_linear": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int,
                            c_int, c_int, _P, c_int, c_int64, c_int, _P, c_int, c_int64, _P, c_int64,
                            _P]),
+    "bfa_build_paged_kv_batch": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int, _P, c_int, c_int64,
+                                         c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "bfa_qk_norm_rope": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, _P, c_int,
+                                 c_int64, c_int64, _P, _P, c_int, c_float, _P, c_int, _P, c_int64, _P, _P]),
+    "bfa_append_paged_kv_fp4": (c_int, [_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                        c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                        c_int64, c_int64, c_int64, c_int64, _P, c_int, c_int64, _P, _P, c_int,
+                                        c_int64, _P, c_int, _P, _P]),
+    "bfa_gather_paged_kv_fp4": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                        c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int, c_int64, _P,
+                                        _P, c_int, c_int64, _P, c_int, c_int64, _P, _P, c_int, _P, _P]),
+    "bfa_paged_attention_workspace_size": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                                     c_int64, c_int64, c_int64, c_int]),
+    "bfa_paged_attention": (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int64, _P, c_int, c_int64, c_int64,
+                                    c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int64, c_int64,
+                                    c_int64, c_int64, _P, c_int64, _P, _P, _P, c_int64, c_float, c_int64,
+                                    c_int64, _P, c_int64, _P, c_int64, _P, _P]),
 }
 
 _lib = None
@@ -341,6 +359,27 @@ def stream_of(device: torch.device):
     if _raw_stream is not None:
         return _raw_stream(idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """A context in which launches go to `device`: its default stream's handle is null,
+    which a launch takes for the current device's.  torch.cuda.device() where it is
+    another one, and nothing (it takes 3 us) where it is current."""
+    idx = device.index
+    return _HERE if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 _status: dict[int, torch.Tensor] = {}

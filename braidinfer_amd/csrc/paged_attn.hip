@@ -1,0 +1,1045 @@
+// Attention of a ragged batch over one paged cache on gfx950, with a sliding
+// window and a few first tokens that stay visible, the cache in 16 bits or in 4.
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale q_r . k_j - max_j)
+//
+// over the keys j that row r sees (bfa_paged.h); a row that sees none is 0.  A row
+// is a query token and one of the Hq / Hkv query heads of a kv head, so a key that
+// is read serves all of them.  Scores, maxima, sums and accumulators are fp32; the
+// weights p are rounded to the queries' 16-bit type for the matrix product (at most
+// half a step, 2^-8 of p in bf16 and 2^-11 in fp16, and the row's largest p is exactly 1).
+//
+// The 4-bit cache holds E2M1 codes, two to a byte, and a power-of-two scale (E8M0)
+// for each 32 elements of a row.  v_cvt_scalef32_pk_bf16_fp4 gives two elements'
+// bf16 values, scale included, exactly; in fp16 the scale is taken 2^-4 times (a
+// value of 4 x 2^14, which an fp16 key of 57344 and more has, is past fp16) and
+// scores and output 2^4 times.
+//
+// The matrix work is done transposed, S^T = K Q^T and O^T = V^T P^T, with
+// v_mfma_f32_16x16x32: a lane owns one row (lane % 16), its maximum and its sum,
+// and P^T is the second product's B operand in the registers that hold it.  V^T
+// comes from the row-major V tile in the LDS by the transposing reads
+// (ds_read_b64_tr_b16: of 16 lanes, lane s passes the address of row s / 4,
+// elements 4 (s % 4) .. +3, and gets element s of each of the four rows).
+//
+// Work is cut by the device itself (locate below), from the lengths that only it
+// needs to know: an item is a block of rows and a range of its key tiles, so that
+// one long request among short ones, or a few rows over a long cache, still fill
+// the chip, and a captured graph follows the lengths of each replay.
+#include <limits.h>
+
+#include <type_traits>
+
+#include "bfa_device.h"
+#include "bfa_host.h"
+#include "bfa_paged.h"
+
+namespace bfa {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 pa_bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 pa_f16x8_t;
+typedef __attribute__((ext_vector_type(4))) float pa_f32x4_t;
+typedef __attribute__((ext_vector_type(4))) short pa_s16x4_t;
+typedef __attribute__((address_space(3))) pa_s16x4_t pa_lds_s16x4_t;
+
+struct PagedArgs {
+  const uint16_t* q;  // [tokens, Hq, D], token / head strides
+  int64_t q_st, q_sh;
+  const uint8_t* cache;           // 16-bit elements, or codes
+  uint32_t c_sp, c_ss;            // page, slot strides in 16-byte units
+  int64_t c_skv, c_sh;            // K|V, head strides in bytes
+  const uint8_t* scales;          // of the 4-bit cache
+  uint32_t s_sp, s_ss;            // its strides in bytes
+  int64_t s_skv, s_sh;
+  int64_t num_pages;
+  const int32_t* indices;
+  int64_t num_indices;
+  const int32_t* kv_indptr;
+  const int32_t* last;
+  const int32_t* qo_indptr;
+  int32_t num_seqs;
+  int64_t tokens;
+  uint32_t hq, hkv;
+  FastDiv group, ps, heads;       // Hq / Hkv, page size, Hkv
+  float sl2, oscale;              // scale x log2(e), factor of the output
+  int32_t window, sinks;
+  uint16_t* out;                  // [tokens, Hq * D], row stride out_st
+  int64_t out_st;
+  int32_t split, target, least;   // 0: an item is a block
+  int32_t nblocks;                // bound of the blocks
+  float* acc;                     // [items, Hkv, BM, D] partial sums
+  float* ml;                      // [items, Hkv, BM, 2] their maxima and sums
+  int4* table;                    // [nblocks] (first item, items, first query row, rows) of a block
+  int* status;
+};
+
+template <bool BF16>
+__device__ __forceinline__ pa_f32x4_t pa_mfma(const uint4& a, const uint4& b, pa_f32x4_t c) {
+  if constexpr (BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8_t, a),
+                                                   __builtin_bit_cast(pa_bf16x8_t, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_f16x8_t, a),
+                                                  __builtin_bit_cast(pa_f16x8_t, b), c, 0, 0, 0);
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  if constexpr (BF16) {
+    return pack_bf16x2(lo, hi);
+  } else {
+    return static_cast<uint32_t>(f32_to_f16_bits(lo)) | (static_cast<uint32_t>(f32_to_f16_bits(hi)) << 16);
+  }
+}
+
+// 8 codes (a dword, the first element in the low 4 bits) as 16-bit values times the
+// power of two in `scale`'s exponent
+template <bool BF16>
+__device__ __forceinline__ uint4 pa_from4(uint32_t w, float scale) {
+  if constexpr (BF16) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3)));
+  } else {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3)));
+  }
+}
+// a scale byte as the float whose exponent the conversion takes; 255 stands for NaN
+template <bool BF16>
+__device__ __forceinline__ float pa_scale(uint32_t byte) {
+  if constexpr (!BF16) byte = byte == 255u ? 255u : byte < 4u ? 0u : byte - 4u;
+  return __uint_as_float(byte << 23);
+}
+
+// whether a word holds a 16-bit infinity or NaN
+template <bool BF16>
+__device__ __forceinline__ bool pa_nonfinite(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+template <bool BF16>
+__device__ __forceinline__ bool pa_nonfinite(const uint4& v) {
+  return pa_nonfinite<BF16>(v.x) || pa_nonfinite<BF16>(v.y) || pa_nonfinite<BF16>(v.z) || pa_nonfinite<BF16>(v.w);
+}
+
+// word j of a quarter row of codes (8 or 16 bytes)
+__device__ __forceinline__ uint32_t pa_word(const uint4& c, int j) { return j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w; }
+__device__ __forceinline__ uint32_t pa_word(const uint2& c, int j) { return j == 0 ? c.x : c.y; }
+
+// ------------------------------------------------------------------- tiles
+// A K or V tile in the LDS: rows of GK = D / 8 granules of 16 bytes.  Granule G of
+// row r is at slot G ^ f(r).  K: the 16 rows of a fragment read then meet in no bank
+// (as 256-byte rows, 64 banks: all of G; as 128-byte rows, two to the 256 bytes,
+// r / 2).  V: of a transposing read's four rows, two granules each, no pair meets,
+// and neither do the four rows of a write of the 4-bit form, a quarter row a lane.
+template <int D>
+__device__ __forceinline__ int k_slot(int r, int G) {
+  if constexpr (D == 128) return G ^ (r & 15);
+  else return G ^ ((r >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int r, int G) {
+  if constexpr (D == 128) return G ^ (((r >> 1) & 1) * 5 | (r & 1) << 1 | ((r >> 2) & 1) << 3);
+  else return G ^ (((r >> 1) & 3) << 1);
+}
+
+// The V^T operand of 32 keys and 16 head-dim columns (block jd), key position 4 b + i
+// of lane group g holding key 16 b + 4 g + i, which is where S^T left its score.
+template <int D>
+__device__ __forceinline__ uint4 v_fragment(const uint4* tile, int key0, int jd, int lane) {
+  constexpr int GK = D / 8;
+  const int s = lane & 15, r = key0 + 4 * (lane >> 4) + (s >> 2);
+  const int G = 2 * jd + ((s & 3) >> 1);
+  uint2 w[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint2* p = reinterpret_cast<const uint2*>(tile + (r + 16 * b) * GK + v_slot<D>(r + 16 * b, G)) + (s & 1);
+    w[b] = __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4_t*)(const_cast<uint2*>(p))));
+  }
+  return make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+}
+
+// Softmax and O^T += V^T P^T of one tile of 16 KC keys for RB blocks of 16 rows;
+// sc: the masked, scaled (base 2) scores of keys 16 c + 4 (lane / 16) + i.
+// `careful`: V holds an infinity or NaN and not every row sees every key, so
+// that a product with a weight of 0 must not happen.
+template <bool BF16, int D, int KC, int RB>
+__device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float (&m)[RB], float (&l)[RB],
+                                       pa_f32x4_t (&o)[RB][D / 16], const uint4* vt, int lane, bool careful) {
+  constexpr int OJ = D / 16;
+  uint4 pf[RB][KC / 2];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[rb][c][i]);
+    mx = lanes4_max(mx);
+    if (__any(mx > m[rb])) {
+      const float top = fmaxf(m[rb], mx);
+      const float alpha = __builtin_amdgcn_exp2f(m[rb] - (top == -INFINITY ? 0.f : top));
+      m[rb] = top;
+      l[rb] *= alpha;
+#pragma unroll
+      for (int j = 0; j < OJ; ++j) o[rb][j] *= alpha;
+    }
+    const float ref = m[rb] == -INFINITY ? 0.f : m[rb];
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[rb][c][i] = __builtin_amdgcn_exp2f(sc[rb][c][i] - ref);
+        sum += sc[rb][c][i];
+      }
+    l[rb] += sum;
+#pragma unroll
+    for (int h = 0; h < KC / 2; ++h)
+      pf[rb][h] = make_uint4(pa_pack<BF16>(sc[rb][2 * h][0], sc[rb][2 * h][1]),
+                             pa_pack<BF16>(sc[rb][2 * h][2], sc[rb][2 * h][3]),
+                             pa_pack<BF16>(sc[rb][2 * h + 1][0], sc[rb][2 * h + 1][1]),
+                             pa_pack<BF16>(sc[rb][2 * h + 1][2], sc[rb][2 * h + 1][3]));
+  }
+  if (!careful) {
+#pragma unroll
+    for (int h = 0; h < KC / 2; ++h)
+#pragma unroll
+      for (int j = 0; j < OJ; ++j) {
+        const uint4 vf = v_fragment<D>(vt, 32 * h, j, lane);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) o[rb][j] = pa_mfma<BF16>(vf, pf[rb][h], o[rb][j]);
+      }
+    return;
+  }
+  // key by key, a lane's columns 16 j + 4 (lane / 16) + i of its row
+  const uint16_t* v16 = reinterpret_cast<const uint16_t*>(vt);
+  for (int g = 0; g < 4; ++g) {
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * c + 4 * g + i;
+        float p[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) p[rb] = __shfl(sc[rb][c][i], (lane & 15) + 16 * g);
+#pragma unroll
+        for (int j = 0; j < OJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 16 * j + 4 * (lane >> 4) + e;
+            const float v = Elem<BF16 ? BFA_DTYPE_BF16 : BFA_DTYPE_F16>::to_f32(
+                v16[(key * (D / 8) + v_slot<D>(key, d >> 3)) * 8 + (d & 7)]);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+              if (p[rb] != 0.f) o[rb][j][e] += p[rb] * v;
+          }
+      }
+  }
+}
+
+// Scores times the scale; where `edge`, those of keys that a row does not see -inf
+// whatever they were.  hi: the row's position, lo: the first key of its window.
+template <int KC, int RB>
+__device__ __forceinline__ void weigh(pa_f32x4_t (&sc)[RB][KC], float sl2, bool edge, int key0,
+                                      const int32_t (&hi)[RB], const int32_t (&lo)[RB], int32_t sinks, int lane) {
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) sc[rb][c] *= sl2;
+  if (!edge) return;
+#pragma unroll
+  for (int c = 0; c < KC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t key = key0 + 16 * c + 4 * (lane >> 4) + i;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        if (key > hi[rb] || (key < lo[rb] && key >= sinks)) sc[rb][c][i] = -INFINITY;
+    }
+}
+
+// first key of the window of a row at position p
+__device__ __forceinline__ int32_t window_from(int32_t p, int32_t window) {
+  return window > 0 && p >= window ? p - window + 1 : 0;
+}
+
+// Whether rows at positions first .. last see the keys key0 .. key0 + n - 1
+// differently: not all of them see all.
+__device__ __forceinline__ bool tile_edge(int32_t key0, int n, int32_t first, int32_t last, int32_t window,
+                                          int32_t sinks) {
+  if (key0 + n - 1 > first) return true;
+  return key0 < window_from(last, window) && key0 + n > sinks;
+}
+
+// ------------------------------------------------------------------- items
+struct Item {
+  PagedSeq s;
+  int32_t block, chunk, chunks, per, index;
+  bool live;
+};
+
+// Inclusive sum over the lanes, held at SCAN_MOST: no request order, broken offsets
+// included, overflows it.  before(): what the lanes before hold.
+constexpr int32_t SCAN_MOST = 0x3fffffff;
+__device__ __forceinline__ int32_t scan_lanes(int32_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int32_t u = __shfl_up(v, d);
+    if (lane >= d) v = min(v + u, SCAN_MOST);
+  }
+  return v;
+}
+__device__ __forceinline__ int32_t before(int32_t end, int lane) {
+  const int32_t u = __shfl_up(end, 1);
+  return lane == 0 ? 0 : u;
+}
+
+// Item x of the grid: every wave finds it by itself, 64 requests at a time, lane by
+// lane.  The first pass sums the work (the key tiles of all blocks), from which the
+// tiles to an item follow; the second finds the request that owns item x.  The
+// item's first workgroup fills the block's line of the table that the merge reads,
+// and workgroups past the last item the lines past the last block.
+template <int BM, int KT>
+__device__ __forceinline__ Item locate(const PagedArgs& a, int32_t x, bool writes_table) {
+  const int lane = threadIdx.x & 63;
+  const int32_t group = static_cast<int32_t>(a.group.d);
+  auto request = [&](int32_t b, bool& bad) {
+    bad = false;
+    PagedSeq s{0, 0, 0, 0, 0};
+    if (b < a.num_seqs)
+      s = paged_seq(a.qo_indptr[b], a.qo_indptr[b + 1], a.kv_indptr[b], a.kv_indptr[b + 1], a.last[b], a.tokens,
+                    a.num_indices, static_cast<int32_t>(a.ps.d), bad);
+    return s;
+  };
+  bool bad;
+  PagedSeq s = request(lane, bad);
+  PagedSplit sp = paged_split(s, group, BM, a.window, a.sinks, KT);
+  int32_t per = INT_MAX;
+  if (a.split) {
+    int64_t total = static_cast<int64_t>(sp.blocks) * sp.tiles;
+    for (int32_t b = 64 + lane; b - lane < a.num_seqs; b += 64) {
+      bool ignored;
+      const PagedSplit q = paged_split(request(b, ignored), group, BM, a.window, a.sinks, KT);
+      total += static_cast<int64_t>(q.blocks) * q.tiles;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    per = paged_per_item(total, a.target, a.least);
+  }
+  Item it{};
+  it.per = per;
+  int32_t items = 0, blocks = 0;  // of the requests before
+  for (int32_t b = lane;; b += 64) {
+    if (b != lane) {
+      s = request(b, bad);
+      sp = paged_split(s, group, BM, a.window, a.sinks, KT);
+    }
+    if (bad && x == 0 && writes_table) flag_status(a.status, BFA_STATUS_INDEX_OOB);
+    const int32_t chunks = sp.chunks(per);
+    const int32_t mine = static_cast<int32_t>(min<int64_t>(static_cast<int64_t>(sp.blocks) * chunks, SCAN_MOST));
+    const int32_t end = scan_lanes(mine, lane), start = before(end, lane);
+    const int32_t bend = scan_lanes(sp.blocks, lane), bstart = before(bend, lane);
+    const uint64_t owner = __ballot(x - items >= start && x - items < end);
+    if (owner) {
+      const int src = __builtin_ctzll(owner);
+      auto rd = [&](int32_t v) { return __builtin_amdgcn_readlane(v, src); };
+      it.s = PagedSeq{rd(s.q0), rd(s.qlen), rd(s.page0), rd(s.npages), rd(s.kvlen)};
+      it.chunks = rd(chunks);
+      const int32_t in = x - items - rd(start);
+      it.block = in / it.chunks;
+      it.chunk = in - it.block * it.chunks;
+      it.index = x;
+      it.live = true;
+      // (read out here, where every lane is active: the compiler may compute what a lane
+      // read gives away under the branch that uses it)
+      const int32_t at = blocks + rd(bstart) + it.block;
+      if (a.split && writes_table && it.chunk == 0 && threadIdx.x == 0) {
+        const int32_t row0 = it.block * BM;
+        if (at < a.nblocks)
+          a.table[at] = make_int4(x, it.chunks, it.s.q0 * group + row0,
+                                  static_cast<int32_t>(min<int64_t>(BM, static_cast<int64_t>(it.s.qlen) * group - row0)));
+      }
+      return it;
+    }
+    items = min(items + __builtin_amdgcn_readlane(end, 63), SCAN_MOST);
+    blocks = min(blocks + __builtin_amdgcn_readlane(bend, 63), SCAN_MOST);
+    if (b - lane + 64 >= a.num_seqs) break;
+  }
+  if (a.split && writes_table && threadIdx.x == 0) {
+    const int64_t at = static_cast<int64_t>(blocks) + (x - items);
+    if (at < a.nblocks) a.table[at] = make_int4(0, 0, 0, 0);
+  }
+  return it;
+}
+
+// The rows of a block: positions and query addresses.
+struct Rows {
+  int32_t row0, n;            // rows of the request, of the block
+  int32_t first, last;        // positions of its first and last row
+};
+template <int BM>
+__device__ __forceinline__ Rows block_rows(const PagedArgs& a, const Item& it) {
+  Rows r;
+  r.row0 = it.block * BM;
+  r.n = static_cast<int32_t>(min<int64_t>(BM, static_cast<int64_t>(it.s.qlen) * a.group.d - r.row0));
+  const int32_t base = it.s.kvlen - it.s.qlen;
+  r.first = base + static_cast<int32_t>(a.group.div(r.row0));
+  r.last = base + static_cast<int32_t>(a.group.div(r.row0 + r.n - 1));
+  return r;
+}
+
+// Address of a key: offsets of its row in the cache (16-byte units) and, in the
+// 4-bit cache, of its scales; ok: the key exists.
+struct KeyRow {
+  uint32_t off, soff;
+  bool ok;
+};
+__device__ __forceinline__ int32_t key_entry(const PagedArgs& a, const PagedSeq& s, int32_t key) {
+  key = max(min(key, s.kvlen - 1), 0);  // (the caller has keys: kvlen > 0)
+  return a.indices[s.page0 + static_cast<int32_t>(a.ps.div(key))];
+}
+template <bool FP4>
+__device__ __forceinline__ KeyRow key_row(const PagedArgs& a, const PagedSeq& s, int32_t key, int32_t id) {
+  KeyRow r{0, 0, key < s.kvlen};
+  const int64_t page = paged_page(id, a.num_pages);
+  if (r.ok && page < 0) {
+    flag_status(a.status, BFA_STATUS_INDEX_OOB);
+    r.ok = false;
+  }
+  if (r.ok) {
+    const uint32_t slot = static_cast<uint32_t>(key) - a.ps.div(key) * a.ps.d;
+    r.off = static_cast<uint32_t>(page) * a.c_sp + slot * a.c_ss;
+    if constexpr (FP4) r.soff = static_cast<uint32_t>(page) * a.s_sp + slot * a.s_ss;
+  }
+  return r;
+}
+__device__ __forceinline__ uint4 zero_unless(bool ok, const uint4& v) {
+  return make_uint4(ok ? v.x : 0u, ok ? v.y : 0u, ok ? v.z : 0u, ok ? v.w : 0u);
+}
+__device__ __forceinline__ uint2 zero_unless(bool ok, const uint2& v) { return make_uint2(ok ? v.x : 0u, ok ? v.y : 0u); }
+
+// ------------------------------------------------------------------ decode
+// Blocks of 16 rows, one kv head, 4 waves: wave w takes key tiles w, w + 4, ... of
+// the item by itself, with its own running state, and the four meet in the LDS at
+// the end.  K fragments go from the cache straight to the registers that the
+// product reads; V goes through the wave's own LDS tile, for the transposing reads.
+// The next tile's rows are in flight during a tile's work, and the page ids of the
+// one after.  Bound by the cache's bytes.
+template <bool BF16, int D, bool FP4>
+__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
+  constexpr int KT = FP4 ? 64 : 32, KC = KT / 16;
+  constexpr int GK = D / 8, QJ = D / 32, OJ = D / 16;
+  constexpr int VN = FP4 ? KT / 16 : KT * GK / 64;  // V loads of a lane: a quarter row of codes, or a granule
+  using Code = std::conditional_t<FP4 && D == 64, uint2, uint4>;  // a quarter row of codes, or a granule
+  __shared__ uint4 vbuf[4][KT * GK];
+  __shared__ float2 state[4][16];
+
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t x = a.heads.div(blockIdx.x), h = blockIdx.x - x * a.hkv;
+  const Item it = locate<16, KT>(a, static_cast<int32_t>(x), h == 0);
+  if (!it.live) return;
+  const Rows rows = block_rows<16>(a, it);
+  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
+  const int32_t i0 = it.chunks > 1 ? it.chunk * it.per : 0;
+  const int32_t i1 = it.chunks > 1 ? min(i0 + it.per, kt.count) : kt.count;
+
+  // this lane's row: its query, as the B operand of S^T, and its position
+  uint4 qf[QJ];
+  int32_t hi[1], lo[1];
+  {
+    const uint32_t r = rows.row0 + min(lane & 15, rows.n - 1), t = a.group.div(r);
+    const uint16_t* qrow =
+        a.q + (it.s.q0 + static_cast<int64_t>(t)) * a.q_st + (h * a.group.d + (r - t * a.group.d)) * a.q_sh;
+    // (the 4-bit form's lane holds columns D / 4 (lane / 16) .. of a key, which then
+    // are its columns of the query)
+#pragma unroll
+    for (int j = 0; j < QJ; ++j)
+      qf[j] = *reinterpret_cast<const uint4*>(qrow + (FP4 ? D / 4 * g4 + 8 * j : 32 * j + 8 * g4));
+    hi[0] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
+    lo[0] = window_from(hi[0], a.window);
+  }
+
+  float m[1] = {-INFINITY}, l[1] = {0.f};
+  pa_f32x4_t o[1][OJ];
+#pragma unroll
+  for (int j = 0; j < OJ; ++j) o[0][j] = pa_f32x4_t{};
+
+  const uint8_t* kbase = a.cache + h * a.c_sh;
+  const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh : nullptr;
+  struct Tile {
+    uint4 k[FP4 ? 1 : KC][FP4 ? 1 : QJ];
+    Code kc[FP4 ? KC : 1], v[VN];
+    uint32_t ks[FP4 ? KC : 1], vs[FP4 ? VN : 1];
+    uint32_t ok;  // of the rows of v
+  };
+  // lane l resolves key l % KT of a tile; its loads take the rows from there
+  auto entry = [&](int32_t i) { return key_entry(a, it.s, kt.at(min(i, kt.count - 1)) * KT + (lane & (KT - 1))); };
+  auto issue = [&](int32_t i, int32_t id) {
+    Tile t;
+    const KeyRow kr = key_row<FP4>(a, it.s, kt.at(i) * KT + (lane & (KT - 1)), id);
+    const uint64_t okay = __ballot(kr.ok);
+    t.ok = 0;
+    if constexpr (FP4) {
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint32_t off = __shfl(kr.off, 16 * c + (lane & 15)), soff = __shfl(kr.soff, 16 * c + (lane & 15));
+        t.kc[c] = *reinterpret_cast<const Code*>(kbase + static_cast<uint64_t>(off) * 16 + D / 8 * g4);
+        t.ks[c] = ksc[static_cast<uint64_t>(soff) + D / 4 * g4 / 32];
+      }
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const int r = 16 * i + (lane >> 2);
+        const uint32_t off = __shfl(kr.off, r), soff = __shfl(kr.soff, r);
+        t.v[i] = *reinterpret_cast<const Code*>(kbase + a.c_skv + static_cast<uint64_t>(off) * 16 + D / 8 * (lane & 3));
+        t.vs[i] = ksc[a.s_skv + static_cast<uint64_t>(soff) + D / 4 * (lane & 3) / 32];
+        t.ok |= static_cast<uint32_t>((okay >> r) & 1) << i;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint32_t off = __shfl(kr.off, 16 * c + (lane & 15));
+        const uint8_t* row = kbase + static_cast<uint64_t>(off) * 16 + 16 * g4;
+#pragma unroll
+        for (int j = 0; j < QJ; ++j) t.k[c][j] = *reinterpret_cast<const uint4*>(row + 64 * j);
+      }
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const int r = 64 / GK * i + lane / GK;
+        const uint32_t off = __shfl(kr.off, r);
+        t.v[i] = *reinterpret_cast<const uint4*>(kbase + a.c_skv + static_cast<uint64_t>(off) * 16 + 16 * (lane % GK));
+        t.ok |= static_cast<uint32_t>((okay >> r) & 1) << i;
+      }
+    }
+    return t;
+  };
+
+  uint4* vt = vbuf[wid];
+  int32_t i = i0 + wid;
+  if (i < i1) {
+    Tile cur = issue(i, entry(i));
+    int32_t id = entry(i + 4);
+    for (; i < i1; i += 4) {
+      const int32_t key0 = kt.at(i) * KT;
+      const bool edge = tile_edge(key0, KT, rows.first, rows.last, a.window, a.sinks);
+      const int32_t id2 = entry(i + 8);
+      Tile nxt;
+      if (i + 4 < i1) nxt = issue(i + 4, id);
+      id = id2;
+      // S^T = K Q^T
+      pa_f32x4_t sc[1][KC];
+#pragma unroll
+      for (int c = 0; c < KC; ++c) sc[0][c] = pa_f32x4_t{};
+#pragma unroll
+      for (int j = 0; j < QJ; ++j)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          if constexpr (FP4) {
+            sc[0][c] = pa_mfma<BF16>(pa_from4<BF16>(pa_word(cur.kc[c], j), pa_scale<BF16>(cur.ks[c])), qf[j], sc[0][c]);
+          } else {
+            sc[0][c] = pa_mfma<BF16>(cur.k[c][j], qf[j], sc[0][c]);
+          }
+        }
+      weigh<KC, 1>(sc, a.sl2, edge, key0, hi, lo, a.sinks, lane);
+      // V -> LDS; rows that do not exist as zeros, since 0 x a NaN would poison the sum
+      bool odd = false;
+      __builtin_amdgcn_wave_barrier();
+      if constexpr (FP4) {
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+          const int r = 16 * i + (lane >> 2);
+          const bool ok = (cur.ok >> i) & 1;
+          const Code c = zero_unless(ok, cur.v[i]);
+          const float s = ok ? pa_scale<BF16>(cur.vs[i]) : 1.f;
+#pragma unroll
+          for (int k = 0; k < QJ; ++k) {
+            const uint4 x = pa_from4<BF16>(pa_word(c, k), s);
+            vt[r * GK + v_slot<D>(r, QJ * (lane & 3) + k)] = x;
+            if (edge && pa_nonfinite<BF16>(x)) odd = true;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+          const int r = 64 / GK * i + lane / GK;
+          const uint4 x = zero_unless((cur.ok >> i) & 1, cur.v[i]);
+          vt[r * GK + v_slot<D>(r, lane % GK)] = x;
+          if (edge && pa_nonfinite<BF16>(x)) odd = true;
+        }
+      }
+      asm volatile("" ::: "memory");  // (one wave's LDS accesses happen in order)
+      __builtin_amdgcn_wave_barrier();
+      attend<BF16, D, KC, 1>(sc, m, l, o, vt, lane, __any(odd));
+      asm volatile("" ::: "memory");
+      cur = nxt;
+    }
+  }
+
+  // the four waves' states meet: granule G (4 columns) of row r at slot G ^ r
+  l[0] = lanes4_sum(l[0]);
+  float4* ob = reinterpret_cast<float4*>(vt);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < OJ; ++j)
+    ob[(lane & 15) * (D / 4) + ((4 * j + g4) ^ (lane & 15))] = make_float4(o[0][j][0], o[0][j][1], o[0][j][2], o[0][j][3]);
+  if (lane < 16) state[wid][lane] = make_float2(m[0], l[0]);
+  __syncthreads();
+  const int r = tid >> 4;  // 16 lanes a row, D / 16 columns each
+  if (r >= rows.n) return;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, state[w][r].x);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 acc[D / 64] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 st = state[w][r];
+    const float f = __builtin_amdgcn_exp2f(st.x - ref);
+    sum += f * st.y;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      const float4 v = reinterpret_cast<const float4*>(vbuf[w])[r * (D / 4) + ((D / 64 * (tid & 15) + c) ^ r)];
+      acc[c].x += f * v.x; acc[c].y += f * v.y; acc[c].z += f * v.z; acc[c].w += f * v.w;
+    }
+  }
+  if (it.chunks == 1) {
+    const uint32_t rr = rows.row0 + r, t = a.group.div(rr);
+    uint16_t* orow = a.out + (it.s.q0 + static_cast<int64_t>(t)) * a.out_st +
+                     (h * a.group.d + (rr - t * a.group.d)) * static_cast<int64_t>(D) + D / 16 * (tid & 15);
+    const float inv = sum == 0.f ? 0.f : a.oscale / sum;
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint4*>(orow) =
+          make_uint4(pa_pack<BF16>(acc[0].x * inv, acc[0].y * inv), pa_pack<BF16>(acc[0].z * inv, acc[0].w * inv),
+                     pa_pack<BF16>(acc[1].x * inv, acc[1].y * inv), pa_pack<BF16>(acc[1].z * inv, acc[1].w * inv));
+    } else {
+      *reinterpret_cast<uint2*>(orow) =
+          make_uint2(pa_pack<BF16>(acc[0].x * inv, acc[0].y * inv), pa_pack<BF16>(acc[0].z * inv, acc[0].w * inv));
+    }
+  } else {
+    const int64_t slot = (static_cast<int64_t>(it.index) * a.hkv + h) * 16 + r;
+    float4* dst = reinterpret_cast<float4*>(a.acc + slot * D) + D / 64 * (tid & 15);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) dst[c] = acc[c];
+    if ((tid & 15) == 0) reinterpret_cast<float2*>(a.ml)[slot] = make_float2(mx, sum);
+  }
+}
+
+// ----------------------------------------------------------------- prefill
+// Blocks of 64 RB rows, one kv head, 4 waves of 16 RB rows each over the same key
+// tiles of 64, which all of them load into the LDS (two tiles: the next one's rows
+// are in flight in registers during a tile's matrix work).  Bound by the matrix
+// cores and the LDS that feeds them.
+template <bool BF16, int D, bool FP4, int RB>
+__global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
+  constexpr int KT = 64, KC = 4, BM = 64 * RB;
+  constexpr int GK = D / 8, QJ = D / 32, OJ = D / 16;
+  constexpr int NL = FP4 ? 1 : GK / 4;  // rows of a tile that a thread loads (a granule, or a quarter row of codes)
+  using Code = std::conditional_t<FP4 && D == 64, uint2, uint4>;
+  __shared__ uint4 kbuf[2][KT * GK];
+  __shared__ uint4 vbuf[2][KT * GK];
+
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t x = a.heads.div(blockIdx.x), h = blockIdx.x - x * a.hkv;
+  // the last blocks of a request see the most keys: they go first
+  const int32_t grid_items = static_cast<int32_t>(a.heads.div(gridDim.x));
+  const Item it = locate<BM, KT>(a, grid_items - 1 - static_cast<int32_t>(x), h == 0);
+  if (!it.live) return;
+  const Rows rows = block_rows<BM>(a, it);
+  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
+  const int32_t i0 = it.chunks > 1 ? it.chunk * it.per : 0;
+  const int32_t i1 = it.chunks > 1 ? min(i0 + it.per, kt.count) : kt.count;
+
+  uint4 qf[RB][QJ];
+  int32_t hi[RB], lo[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const uint32_t r = rows.row0 + min(16 * (RB * wid + rb) + (lane & 15), rows.n - 1), t = a.group.div(r);
+    const uint16_t* qrow =
+        a.q + (it.s.q0 + static_cast<int64_t>(t)) * a.q_st + (h * a.group.d + (r - t * a.group.d)) * a.q_sh;
+#pragma unroll
+    for (int j = 0; j < QJ; ++j) qf[rb][j] = *reinterpret_cast<const uint4*>(qrow + 32 * j + 8 * g4);
+    hi[rb] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
+    lo[rb] = window_from(hi[rb], a.window);
+  }
+  // positions of this wave's first and last row (a wave without rows repeats the last)
+  const int32_t base = it.s.kvlen - it.s.qlen;
+  const int32_t wfirst = base + static_cast<int32_t>(a.group.div(rows.row0 + min(16 * RB * wid, rows.n - 1)));
+  const int32_t wlast = base + static_cast<int32_t>(a.group.div(rows.row0 + min(16 * RB * wid + 16 * RB - 1, rows.n - 1)));
+  const bool idle = 16 * RB * wid >= rows.n;
+
+  float m[RB], l[RB];
+  pa_f32x4_t o[RB][OJ];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int j = 0; j < OJ; ++j) o[rb][j] = pa_f32x4_t{};
+  }
+
+  // staging: row of load n, and this thread's part of a row
+  auto row_of = [&](int n) { return FP4 ? tid >> 2 : tid / GK + 256 / GK * n; };
+  const int part = FP4 ? tid & 3 : tid % GK;
+  const uint8_t* kbase = a.cache + h * a.c_sh + (FP4 ? D / 8 : 16) * part;
+  const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh + D / 4 * part / 32 : nullptr;
+  struct Tile {
+    Code k[NL], v[NL];
+    uint32_t ks, vs;
+    bool ok[NL];
+  };
+  struct Ids {
+    int32_t id[NL];
+  };
+  auto entries = [&](int32_t i) {
+    Ids e;
+    const int32_t key0 = kt.at(min(i, kt.count - 1)) * KT;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) e.id[n] = key_entry(a, it.s, key0 + row_of(n));
+    return e;
+  };
+  auto issue = [&](int32_t i, const Ids& e) {
+    Tile t;
+    const int32_t key0 = kt.at(i) * KT;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const KeyRow kr = key_row<FP4>(a, it.s, key0 + row_of(n), e.id[n]);
+      const uint8_t* p = kbase + static_cast<uint64_t>(kr.off) * 16;
+      t.k[n] = *reinterpret_cast<const Code*>(p);
+      t.v[n] = *reinterpret_cast<const Code*>(p + a.c_skv);
+      if constexpr (FP4) {
+        t.ks = ksc[kr.soff];
+        t.vs = ksc[a.s_skv + kr.soff];
+      }
+      t.ok[n] = kr.ok;
+    }
+    return t;
+  };
+  // a tile into the LDS, rows that do not exist as zeros; whether its V holds an
+  // infinity or NaN, asked where some row does not see all of it
+  auto store = [&](const Tile& t, int b, bool edge) {
+    bool odd = false;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int r = row_of(n);
+      const Code kc = zero_unless(t.ok[n], t.k[n]), vc = zero_unless(t.ok[n], t.v[n]);
+      if constexpr (FP4) {
+        const float fk = t.ok[n] ? pa_scale<BF16>(t.ks) : 1.f, fv = t.ok[n] ? pa_scale<BF16>(t.vs) : 1.f;
+#pragma unroll
+        for (int k = 0; k < QJ; ++k) {
+          const uint4 xv = pa_from4<BF16>(pa_word(vc, k), fv);
+          kbuf[b][r * GK + k_slot<D>(r, QJ * part + k)] = pa_from4<BF16>(pa_word(kc, k), fk);
+          vbuf[b][r * GK + v_slot<D>(r, QJ * part + k)] = xv;
+          if (edge && pa_nonfinite<BF16>(xv)) odd = true;
+        }
+      } else {
+        kbuf[b][r * GK + k_slot<D>(r, part)] = kc;
+        vbuf[b][r * GK + v_slot<D>(r, part)] = vc;
+        if (edge && pa_nonfinite<BF16>(vc)) odd = true;
+      }
+    }
+    return odd;
+  };
+  auto wg_edge = [&](int32_t i) {
+    return tile_edge(kt.at(i) * KT, KT, rows.first, rows.last, a.window, a.sinks);
+  };
+  // every wave's part of a tile is in the LDS, and every wave is done with the other
+  auto meet = [&](bool edge, bool odd) {
+    if (edge) return __syncthreads_or(odd) != 0;
+    __syncthreads();
+    return false;
+  };
+
+  if (i0 < i1) {
+    Ids id = entries(i0);
+    Tile cur = issue(i0, id);
+    id = entries(i0 + 1);
+    bool careful;
+    {
+      const bool e = wg_edge(i0);
+      careful = meet(e, store(cur, 0, e));
+    }
+    for (int32_t i = i0; i < i1; ++i) {
+      const int b = (i - i0) & 1;
+      const bool more = i + 1 < i1;
+      const Ids id2 = entries(i + 2);
+      if (more) cur = issue(i + 1, id);
+      id = id2;
+      const int32_t key0 = kt.at(i) * KT;
+      // (a wave skips a tile that none of its rows sees)
+      if (!idle && key0 <= wlast && (key0 + KT > window_from(wfirst, a.window) || key0 < a.sinks)) {
+        pa_f32x4_t sc[RB][KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) sc[rb][c] = pa_f32x4_t{};
+#pragma unroll
+        for (int j = 0; j < QJ; ++j)
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            const int r = 16 * c + (lane & 15);
+            const uint4 kf = kbuf[b][r * GK + k_slot<D>(r, 4 * j + g4)];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) sc[rb][c] = pa_mfma<BF16>(kf, qf[rb][j], sc[rb][c]);
+          }
+        weigh<KC, RB>(sc, a.sl2, tile_edge(key0, KT, wfirst, wlast, a.window, a.sinks), key0, hi, lo, a.sinks, lane);
+        attend<BF16, D, KC, RB>(sc, m, l, o, vbuf[b], lane, careful);
+      }
+      if (more) {
+        const bool e = wg_edge(i + 1);
+        careful = meet(e, store(cur, b ^ 1, e));
+      }
+    }
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    l[rb] = lanes4_sum(l[rb]);
+    const int r = 16 * (RB * wid + rb) + (lane & 15);
+    if (r >= rows.n) continue;
+    if (it.chunks == 1) {
+      const uint32_t rr = rows.row0 + r, t = a.group.div(rr);
+      uint16_t* orow = a.out + (it.s.q0 + static_cast<int64_t>(t)) * a.out_st +
+                       (h * a.group.d + (rr - t * a.group.d)) * static_cast<int64_t>(D) + 4 * g4;
+      const float inv = l[rb] == 0.f ? 0.f : a.oscale / l[rb];
+#pragma unroll
+      for (int j = 0; j < OJ; ++j)
+        *reinterpret_cast<uint2*>(orow + 16 * j) = make_uint2(pa_pack<BF16>(o[rb][j][0] * inv, o[rb][j][1] * inv),
+                                                              pa_pack<BF16>(o[rb][j][2] * inv, o[rb][j][3] * inv));
+    } else {
+      const int64_t slot = (static_cast<int64_t>(it.index) * a.hkv + h) * BM + r;
+      float4* dst = reinterpret_cast<float4*>(a.acc + slot * D) + g4;
+#pragma unroll
+      for (int j = 0; j < OJ; ++j) dst[4 * j] = make_float4(o[rb][j][0], o[rb][j][1], o[rb][j][2], o[rb][j][3]);
+      if (lane < 16) reinterpret_cast<float2*>(a.ml)[slot] = make_float2(m[rb], l[rb]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- merge
+// Joins the items of each block that has several: a group of D / 4 lanes takes 4
+// columns each of every (64 / (D / 4))-th item of a row, the groups of a wave meet
+// by lane swaps, in one order whatever runs first.
+template <bool BF16, int D, int BM>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  constexpr int L = D / 4, NG = 64 / L, U = 8;
+  const uint32_t block = a.heads.div(blockIdx.x), h = blockIdx.x - block * a.hkv;
+  const int4 line = a.table[block];
+  const int32_t items = line.y, n = line.w;
+  if (items <= 1) return;
+  const int lane = threadIdx.x & 63, sub = lane / L, col = lane % L;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < n; r += 4 * gridDim.y) {
+    const int64_t slot0 = (static_cast<int64_t>(line.x) * a.hkv + h) * BM + r, step = static_cast<int64_t>(a.hkv) * BM;
+    const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot0;
+    float mx = -INFINITY;
+    for (int z = lane; z < items; z += 64) mx = fmaxf(mx, ml[z * step].x);
+    mx = lanes4_max(group16_max_dpp(mx));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    float4 acc = {};
+    for (int z0 = 0; z0 < items; z0 += NG * U) {
+      float2 st[U];
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int z = min(z0 + NG * u + sub, items - 1);
+        st[u] = ml[z * step];
+        v[u] = reinterpret_cast<const float4*>(a.acc + (slot0 + z * step) * D)[col];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (z0 + NG * u + sub >= items) continue;
+        const float f = __builtin_amdgcn_exp2f(st[u].x - ref);
+        sum += f * st[u].y;
+        acc.x += f * v[u].x; acc.y += f * v[u].y; acc.z += f * v[u].z; acc.w += f * v[u].w;
+      }
+    }
+#pragma unroll
+    for (int d = L; d < 64; d *= 2) {
+      sum += __shfl_xor(sum, d);
+      acc.x += __shfl_xor(acc.x, d); acc.y += __shfl_xor(acc.y, d);
+      acc.z += __shfl_xor(acc.z, d); acc.w += __shfl_xor(acc.w, d);
+    }
+    if (sub) continue;
+    const float inv = sum == 0.f ? 0.f : a.oscale / sum;
+    const uint32_t rr = static_cast<uint32_t>(line.z) + r, t = a.group.div(rr);
+    uint16_t* orow = a.out + static_cast<int64_t>(t) * a.out_st + (h * a.group.d + (rr - t * a.group.d)) * static_cast<int64_t>(D);
+    reinterpret_cast<uint2*>(orow)[col] =
+        make_uint2(pa_pack<BF16>(acc.x * inv, acc.y * inv), pa_pack<BF16>(acc.z * inv, acc.w * inv));
+  }
+}
+
+// -------------------------------------------------------------------- plan
+struct PagedPlan {
+  int bm, rb;                     // rows of a block; rb 0: the decode form
+  int32_t split, target, least, nblocks, items;
+  int64_t acc_bytes, ml_bytes, table_bytes;
+  int64_t total() const { return acc_bytes + ml_bytes + table_bytes; }
+};
+
+// The form follows the rows of an average request, and the items the workgroups that
+// fill the chip; the lengths themselves stay on the device.
+static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int64_t hkv, int64_t d,
+                            int64_t num_indices, int64_t page_size, int64_t window, int64_t sinks, bool fp4) {
+  PagedPlan p{};
+  const int64_t rows = tokens * group;
+  p.rb = rows <= 16 * num_seqs ? 0 : rows <= 64 * num_seqs ? 1 : 2;
+  p.bm = p.rb == 0 ? 16 : 64 * p.rb;
+  const int64_t kt = p.rb == 0 && !fp4 ? 32 : 64;
+  p.nblocks = static_cast<int32_t>(std::min(rows, rows / p.bm + num_seqs));
+  p.least = p.rb == 0 ? 4 : 2;
+  p.target = static_cast<int32_t>(std::max<int64_t>(1, cdiv(p.rb == 0 ? 1024 : 512, hkv)));
+  int64_t most = cdiv(num_indices * page_size, kt);  // key tiles of a block
+  if (window > 0) most = std::min(most, (window + p.bm / group + 2) / kt + 2 + sinks / kt + 1);
+  p.split = most > p.least && (p.rb == 0 ? p.nblocks * hkv < 8192 : p.nblocks * hkv < 1024);
+  p.items = p.nblocks + (p.split ? p.target : 0);
+  if (p.split) {
+    const int64_t slots = static_cast<int64_t>(p.items) * hkv * p.bm;
+    p.acc_bytes = slots * d * 4;
+    p.ml_bytes = cdiv(slots * 8, 16) * 16;
+    p.table_bytes = static_cast<int64_t>(p.nblocks) * 16;
+  }
+  return p;
+}
+
+static bool paged_head_dim(int64_t d) { return d == 64 || d == 128; }
+
+// what the 32-bit arithmetic of the kernels holds
+static int paged_limits(const char* what, int64_t tokens, int64_t num_seqs, int64_t hq, int64_t hkv, int64_t d,
+                        int64_t num_indices, int64_t page_size) {
+  BFA_REQUIRE(tokens >= 0 && num_seqs >= 0 && hq > 0 && hkv > 0 && num_indices >= 0 && page_size > 0, "%s: bad geometry", what);
+  BFA_REQUIRE(hq % hkv == 0, "%s: %lld query heads do not share %lld kv heads evenly", what,
+              static_cast<long long>(hq), static_cast<long long>(hkv));
+  if (!paged_head_dim(d))
+    return set_error(BFA_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, static_cast<long long>(d));
+  const int64_t lim = int64_t{1} << 31;
+  BFA_REQUIRE(num_seqs < lim / 2 && num_indices < lim && page_size < lim && num_indices * page_size < lim,
+              "%s: 2^31 cached tokens or more", what);
+  BFA_REQUIRE(tokens < lim && hq < lim && tokens * (hq / hkv) < lim / 2 &&
+                  (tokens * (hq / hkv) / 16 + num_seqs + 1024) * hkv < lim / 2,
+              "%s: too many query rows", what);
+  return BFA_OK;
+}
+
+}  // namespace bfa
+
+using namespace bfa;
+
+extern "C" int64_t bfa_paged_attention_workspace_size(int64_t tokens, int64_t num_seqs, int64_t num_q_heads,
+                                                      int64_t num_kv_heads, int64_t head_dim, int64_t num_indices,
+                                                      int64_t page_size, int64_t window, int64_t sinks, int cache_dtype) {
+  if (tokens <= 0 || num_seqs <= 0 ||
+      paged_limits("bfa_paged_attention_workspace_size", tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, num_indices,
+                   page_size) != BFA_OK)
+    return 0;
+  return paged_plan(tokens, num_seqs, num_q_heads / num_kv_heads, num_kv_heads, head_dim, num_indices, page_size, window,
+                    sinks, cache_dtype == BFA_DTYPE_FP4).total();
+}
+
+extern "C" int bfa_paged_attention(
+    const void* query, int dtype, int64_t num_tokens, int64_t num_q_heads, int64_t q_stride_token,
+    int64_t q_stride_head, const void* cache, int cache_dtype, int64_t num_pages, int64_t num_kv_heads,
+    int64_t page_size, int64_t head_dim, int64_t stride_page, int64_t stride_kv, int64_t stride_head,
+    int64_t stride_slot, const void* scales, int64_t scale_stride_page, int64_t scale_stride_kv,
+    int64_t scale_stride_head, int64_t scale_stride_slot, const int32_t* kv_indices, int64_t num_indices,
+    const int32_t* kv_indptr, const int32_t* kv_last_page_len, const int32_t* qo_indptr, int64_t num_seqs,
+    float scale, int64_t window, int64_t sinks, void* out, int64_t out_stride_token, void* workspace,
+    int64_t workspace_bytes, int32_t* status, void* stream) {
+  const char* what = "bfa_paged_attention";
+  BFA_REQUIRE(dtype == BFA_DTYPE_BF16 || dtype == BFA_DTYPE_F16, "%s: queries must be bf16 or fp16", what);
+  const bool fp4 = cache_dtype == BFA_DTYPE_FP4;
+  BFA_REQUIRE(fp4 || cache_dtype == dtype, "%s: the cache must have the queries' dtype, or 4 bits", what);
+  const int rc = paged_limits(what, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, num_indices, page_size);
+  if (rc != BFA_OK) return rc;
+  BFA_REQUIRE(num_pages >= 0 && window >= 0 && sinks >= 0, "%s: negative pages, window or sinks", what);
+  const auto pos = [](int64_t a, int64_t b, int64_t c, int64_t d) { return a >= 0 && b >= 0 && c >= 0 && d >= 0; };
+  BFA_REQUIRE(pos(stride_page, stride_kv, stride_head, stride_slot) &&
+                  (!fp4 || pos(scale_stride_page, scale_stride_kv, scale_stride_head, scale_stride_slot)),
+              "%s: negative cache strides", what);
+  const int64_t unit = fp4 ? 16 : 8;  // elements (bytes of codes) in 16 bytes
+  BFA_REQUIRE(q_stride_token % 8 == 0 && q_stride_head % 8 == 0 && out_stride_token % 8 == 0 &&
+                  stride_page % unit == 0 && stride_kv % unit == 0 && stride_head % unit == 0 && stride_slot % unit == 0 &&
+                  aligned16(query) && aligned16(cache) && aligned16(out) && aligned16(workspace),
+              "%s: tensors must be 16-byte aligned with strides in multiples of 16 bytes", what);
+  if (num_tokens == 0 || num_seqs == 0) return BFA_OK;
+  BFA_REQUIRE(query && out && qo_indptr && kv_indptr && kv_last_page_len, "%s: null pointer", what);
+  BFA_REQUIRE(num_indices == 0 || (kv_indices && cache && (!fp4 || scales) && num_pages > 0), "%s: null cache or page list", what);
+  const int64_t span = num_pages > 0 ? (num_pages - 1) * (stride_page / unit) + (page_size - 1) * (stride_slot / unit) : 0;
+  const int64_t sspan = fp4 && num_pages > 0 ? (num_pages - 1) * scale_stride_page + (page_size - 1) * scale_stride_slot : 0;
+  const int64_t lim32 = int64_t{1} << 32;
+  BFA_REQUIRE(num_pages < (int64_t{1} << 31) && stride_page / unit < lim32 && stride_slot / unit < lim32 && span < lim32 &&
+                  scale_stride_page < lim32 && scale_stride_slot < lim32 && sspan < lim32,
+              "%s: a cache beyond 64 GiB", what);
+  const int64_t win = window >= (int64_t{1} << 31) ? 0 : window;  // (wider than any cache: no window)
+  const int64_t snk = std::min<int64_t>(sinks, (int64_t{1} << 31) - 1);
+  const int64_t group = num_q_heads / num_kv_heads;
+  const PagedPlan p = paged_plan(num_tokens, num_seqs, group, num_kv_heads, head_dim, num_indices, page_size, win, snk, fp4);
+  BFA_REQUIRE(p.total() == 0 || (workspace && workspace_bytes >= p.total()), "%s: workspace too small", what);
+
+  PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(query);
+  a.q_st = q_stride_token; a.q_sh = q_stride_head;
+  a.cache = static_cast<const uint8_t*>(cache);
+  const int64_t bytes = fp4 ? 1 : 2;
+  a.c_sp = static_cast<uint32_t>(stride_page / unit); a.c_ss = static_cast<uint32_t>(stride_slot / unit);
+  a.c_skv = stride_kv * bytes; a.c_sh = stride_head * bytes;
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.s_sp = static_cast<uint32_t>(scale_stride_page); a.s_ss = static_cast<uint32_t>(scale_stride_slot);
+  a.s_skv = scale_stride_kv; a.s_sh = scale_stride_head;
+  a.num_pages = num_pages;
+  a.indices = kv_indices; a.num_indices = num_indices;
+  a.kv_indptr = kv_indptr; a.last = kv_last_page_len; a.qo_indptr = qo_indptr;
+  a.num_seqs = static_cast<int32_t>(num_seqs);
+  a.tokens = num_tokens;
+  a.hq = static_cast<uint32_t>(num_q_heads); a.hkv = static_cast<uint32_t>(num_kv_heads);
+  a.group = FastDiv(static_cast<uint32_t>(group));
+  a.ps = FastDiv(static_cast<uint32_t>(page_size));
+  a.heads = FastDiv(a.hkv);
+  const float back = fp4 && dtype == BFA_DTYPE_F16 ? 16.f : 1.f;
+  a.sl2 = scale * 1.4426950408889634f * back;
+  a.oscale = back;
+  a.window = static_cast<int32_t>(win); a.sinks = static_cast<int32_t>(snk);
+  a.out = static_cast<uint16_t*>(out); a.out_st = out_stride_token;
+  a.split = p.split; a.target = p.target; a.least = p.least; a.nblocks = p.nblocks;
+  char* ws = static_cast<char*>(workspace);
+  a.acc = reinterpret_cast<float*>(ws);
+  a.ml = reinterpret_cast<float*>(ws + p.acc_bytes);
+  a.table = reinterpret_cast<int4*>(ws + p.acc_bytes + p.ml_bytes);
+  a.status = status;
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid(static_cast<unsigned>(p.items * num_kv_heads));
+  auto launch = [&](auto bf, auto dd, auto four) {
+    constexpr bool B = decltype(bf)::value, F = decltype(four)::value;
+    constexpr int DD = decltype(dd)::value;
+    const unsigned blocks = static_cast<unsigned>(p.nblocks * num_kv_heads);
+    if (p.rb == 0) {
+      hipLaunchKernelGGL((paged_decode_kernel<B, DD, F>), grid, dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 16>), dim3(blocks), dim3(256), 0, s, a);
+    } else if (p.rb == 1) {
+      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, 1>), grid, dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 64>), dim3(blocks, 4), dim3(256), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, 2>), grid, dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 128>), dim3(blocks, 8), dim3(256), 0, s, a);
+    }
+  };
+  auto with_d = [&](auto bf, auto four) {
+    if (head_dim == 64) launch(bf, std::integral_constant<int, 64>{}, four);
+    else launch(bf, std::integral_constant<int, 128>{}, four);
+  };
+  if (dtype == BFA_DTYPE_BF16) {
+    if (fp4) with_d(std::true_type{}, std::true_type{}); else with_d(std::true_type{}, std::false_type{});
+  } else {
+    if (fp4) with_d(std::false_type{}, std::true_type{}); else with_d(std::false_type{}, std::false_type{});
+  }
+  return check_launch(what);
+}

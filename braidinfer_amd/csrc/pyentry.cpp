@@ -139,6 +139,12 @@ PyMethodDef methods[] = {
     BFA_ENTRY(bfa_cascade_attention),
     BFA_ENTRY(bfa_linear_workspace_size),
     BFA_ENTRY(bfa_linear),
+    BFA_ENTRY(bfa_build_paged_kv_batch),
+    BFA_ENTRY(bfa_qk_norm_rope),
+    BFA_ENTRY(bfa_append_paged_kv_fp4),
+    BFA_ENTRY(bfa_gather_paged_kv_fp4),
+    BFA_ENTRY(bfa_paged_attention_workspace_size),
+    BFA_ENTRY(bfa_paged_attention),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -31,6 +31,7 @@ extern "C" {
 #define BFA_DTYPE_BF16 2
 #define BFA_DTYPE_I32 3
 #define BFA_DTYPE_I64 4
+#define BFA_DTYPE_FP4 5 /* E2M1 codes, two to a byte, with E8M0 scales (4-bit cache) */
 
 /* return codes */
 #define BFA_OK 0
@@ -486,6 +487,124 @@ int bfa_linear(const void* x, int dtype, int64_t tokens, int64_t k, int64_t x_st
                int mode, int proj_dtype, const void* residual, int residual_dtype, int64_t residual_stride, int sum_dtype,
                void* out, int out_dtype, int64_t out_stride, void* workspace,
                int64_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------- batches of requests --
+ * A step's batch from its requests' lengths, on the device (build_paged_kv_indices,
+ * kernels/kv_cache_utils.py:81-118, and the page manager's position loops,
+ * engine/page_manager.py:159-218, 313-353, build it on the host).
+ * page_tables [num_seqs, max_pages] int32/int64 (row stride page_table_stride),
+ * seq_lens: tokens in the cache after the step, query_lens: the new ones among
+ * them, both [num_seqs] int32/int64.  Writes
+ *   qo_indptr, kv_indptr [num_seqs + 1]: offsets of the requests' tokens and pages;
+ *   kv_indices [num_indices]: their page ids, request by request;
+ *   kv_last_page_len [num_seqs]: tokens on the last page (0 without pages);
+ *   batch_indices, positions, slot_mapping [num_tokens]: each new token's request,
+ *     position seq_len - query_len + i, and slot page id * page_size + position %
+ *     page_size.
+ * kv_indices, batch_indices, positions and slot_mapping hold -1 behind the last
+ * request.  A negative length, a seq_len past the page table, a query_len past the
+ * seq_len, and pages or tokens past num_indices / num_tokens set
+ * BFA_STATUS_INDEX_OOB: the length is then taken as 0, the pages are those of the
+ * table, such tokens have slot -1, and what does not fit is left out. */
+int bfa_build_paged_kv_batch(const void* page_tables, int page_tables_dtype, int64_t num_seqs,
+                             int64_t max_pages, int64_t page_table_stride, const void* seq_lens,
+                             int seq_lens_dtype, const void* query_lens, int query_lens_dtype,
+                             int64_t page_size, int64_t num_tokens, int64_t num_indices,
+                             int32_t* qo_indptr, int32_t* kv_indptr, int32_t* kv_indices,
+                             int32_t* kv_last_page_len, int32_t* batch_indices, int64_t* positions,
+                             int64_t* slot_mapping, int32_t* status, void* stream);
+
+/* RMSNorm of every query and key head and their rotation by position in one pass
+ * (q_norm, k_norm and rotary_emb of models/qwen3.py:257-309, for a q and k that a
+ * projection wrote without them).  query / key [num_tokens, heads, head_dim] (token
+ * / head strides), query_out / key_out contiguous, all of `dtype`:
+ *   x' = x / sqrt(mean(x^2) + eps) * w;  y = (x1' cos - x2' sin, x2' cos + x1' sin)
+ * in fp32, rounded once.  q_norm_weight / k_norm_weight [head_dim] may each be NULL
+ * (no norm); either heads may be 0.  head_dim even.  Positions as in
+ * bfa_rotary_embedding. */
+int bfa_qk_norm_rope(const void* query, int64_t q_heads, int64_t q_stride_token,
+                     int64_t q_stride_head, void* query_out, const void* key, int64_t k_heads,
+                     int64_t k_stride_token, int64_t k_stride_head, void* key_out, int dtype,
+                     int64_t num_tokens, int64_t head_dim, const void* q_norm_weight,
+                     const void* k_norm_weight, int weight_dtype, float eps, const void* positions,
+                     int positions_dtype, const float* cos_sin_cache, int64_t max_position,
+                     int32_t* status, void* stream);
+
+/* Paged append to a cache held in 4 bits (no counterpart in the reference, whose
+ * cache is 16-bit): bfa_append_paged_kv with each block of 32 elements of a head's
+ * row stored as 32 E2M1 codes (two to a byte, the even element in the low bits) and
+ * one byte 127 + e of its scale 2^e, the smallest power of two (from 2^-126) that
+ * keeps the block's largest magnitude within 6; a code is the value over the scale
+ * rounded to nearest even.  A block with an infinity or a NaN gets scale byte 255
+ * and reads as NaN.  codes [num_pages, 2, heads, page_size, head_dim / 2] and scales
+ * [num_pages, 2, heads, page_size, head_dim / 32] bytes, strides (page, K|V, head,
+ * slot) in bytes, those of codes multiples of 4; head_dim a multiple of 32.  Token
+ * addressing as in bfa_append_paged_kv, but with kv_indptr a token whose batch index
+ * is -1 is padding: skipped without a status. */
+int bfa_append_paged_kv_fp4(const void* k, const void* v, int kv_dtype, int64_t num_tokens,
+                            int64_t num_kv_heads, int64_t head_dim, int64_t k_stride_token,
+                            int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
+                            void* codes, void* scales, int64_t num_pages, int64_t page_size,
+                            int64_t stride_page, int64_t stride_kv, int64_t stride_head,
+                            int64_t stride_slot, int64_t scale_stride_page, int64_t scale_stride_kv,
+                            int64_t scale_stride_head, int64_t scale_stride_slot,
+                            const void* kv_indices, int kv_indices_dtype, int64_t num_indices,
+                            const int32_t* kv_indptr, const void* batch_indices,
+                            int batch_indices_dtype, int64_t num_seqs, const void* positions,
+                            int positions_dtype, int32_t* status, void* stream);
+
+/* The values that the 4-bit cache holds for given tokens: k_out, v_out [num_tokens,
+ * heads, head_dim] contiguous, in out_dtype (bf16 and fp32 hold them exactly, but
+ * for 2^128, to which magnitudes from 3.5 x 2^126 round and which reads as infinity;
+ * fp16 within its range).  Tokens addressed as in bfa_append_paged_kv_fp4; one without a
+ * place reads as zeros. */
+int bfa_gather_paged_kv_fp4(const void* codes, const void* scales, int64_t num_pages,
+                            int64_t page_size, int64_t num_kv_heads, int64_t head_dim,
+                            int64_t stride_page, int64_t stride_kv, int64_t stride_head,
+                            int64_t stride_slot, int64_t scale_stride_page, int64_t scale_stride_kv,
+                            int64_t scale_stride_head, int64_t scale_stride_slot,
+                            const void* kv_indices, int kv_indices_dtype, int64_t num_indices,
+                            const int32_t* kv_indptr, const void* batch_indices,
+                            int batch_indices_dtype, int64_t num_seqs, const void* positions,
+                            int positions_dtype, int64_t num_tokens, void* k_out, void* v_out,
+                            int out_dtype, int32_t* status, void* stream);
+
+/* Causal attention of a ragged batch over one paged cache, with a sliding window and
+ * first tokens that stay visible (no counterpart in the reference, whose cascade
+ * attention serves one token stream, layers/cascade_attention.py:50-231).
+ * Request s owns query rows [qo_indptr[s], qo_indptr[s+1]) and the pages
+ * kv_indices[kv_indptr[s] .. kv_indptr[s+1]), the last of which holds
+ * kv_last_page_len[s] tokens; its queries are its last tokens, so that row i stands
+ * at position kv_len - q_len + i and sees key j if j <= position and, with window >
+ * 0, position - j < window or j < sinks.  A row that sees no key (an empty cache, a
+ * position below 0) is 0; rows outside every request are left as they were.
+ * query [num_tokens, Hq, head_dim] bf16 or fp16 (token / head strides), head_dim 64
+ * or 128; query head h attends kv head h / (Hq / Hkv).  cache: one layer of the
+ * queries' dtype, [num_pages, 2, Hkv, page_size, head_dim] by strides (page, K|V,
+ * head, slot) in elements, or with cache_dtype BFA_DTYPE_FP4 the codes and scales of
+ * bfa_append_paged_kv_fp4, strides in bytes.  The cache's and the queries' strides
+ * are multiples of 16 bytes; scales' strides any.  Page ids wrap below 0 as in
+ * bfa_append_paged_kv; a page that does not exist, and offsets outside the arrays,
+ * set BFA_STATUS_INDEX_OOB (the page's keys, the request's rows or keys are left
+ * out).  out [num_tokens, Hq * head_dim], queries' dtype.  num_indices * page_size
+ * and Hq / Hkv * num_tokens below 2^31 and 2^30.  workspace:
+ * bfa_paged_attention_workspace_size bytes, 16-byte aligned. */
+int64_t bfa_paged_attention_workspace_size(int64_t tokens, int64_t num_seqs, int64_t num_q_heads,
+                                           int64_t num_kv_heads, int64_t head_dim,
+                                           int64_t num_indices, int64_t page_size, int64_t window,
+                                           int64_t sinks, int cache_dtype);
+int bfa_paged_attention(const void* query, int dtype, int64_t num_tokens, int64_t num_q_heads,
+                        int64_t q_stride_token, int64_t q_stride_head, const void* cache,
+                        int cache_dtype, int64_t num_pages, int64_t num_kv_heads,
+                        int64_t page_size, int64_t head_dim, int64_t stride_page,
+                        int64_t stride_kv, int64_t stride_head, int64_t stride_slot,
+                        const void* scales, int64_t scale_stride_page, int64_t scale_stride_kv,
+                        int64_t scale_stride_head, int64_t scale_stride_slot,
+                        const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                        const int32_t* kv_last_page_len, const int32_t* qo_indptr,
+                        int64_t num_seqs, float scale, int64_t window, int64_t sinks, void* out,
+                        int64_t out_stride_token, void* workspace, int64_t workspace_bytes,
+                        int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

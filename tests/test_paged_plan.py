@@ -1,0 +1,149 @@
+"""How a ragged batch is cut into key tiles and work items (csrc/bfa_paged.h): built for
+the host and compared with enumeration, broken offsets and page ids among the inputs."""
+from __future__ import annotations
+
+import ctypes
+import random
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "braidinfer_amd" / "csrc"
+SOURCE = r"""
+#include "bfa_paged.h"
+using namespace bfa;
+extern "C" {
+int seq(const int* in, long long tokens, long long indices, int ps, int* out) {
+  bool bad;
+  PagedSeq s = paged_seq(in[0], in[1], in[2], in[3], in[4], tokens, indices, ps, bad);
+  out[0] = s.q0; out[1] = s.qlen; out[2] = s.page0; out[3] = s.npages; out[4] = s.kvlen;
+  return bad;
+}
+long long page(long long id, long long pages) { return paged_page(id, pages); }
+int tiles(int first, int last, int kvlen, int window, int sinks, int tile, int* out) {
+  KeyTiles k = paged_key_tiles(first, last, kvlen, window, sinks, tile);
+  for (int i = 0; i < k.count && i < 4096; ++i) out[i] = k.at(i);
+  return k.count;
+}
+int split(int qlen, int kvlen, int group, int bm, int window, int sinks, int tile, int* blocks) {
+  PagedSeq s{0, qlen, 0, 0, kvlen};
+  PagedSplit p = paged_split(s, group, bm, window, sinks, tile);
+  *blocks = p.blocks;
+  return p.tiles;
+}
+int chunks(int blocks, int tiles, int per) { return PagedSplit{blocks, tiles}.chunks(per); }
+int per_item(long long total, int target, int least) { return paged_per_item(total, target, least); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        pytest.skip("no host C++ compiler")
+    d = tmp_path_factory.mktemp("paged_plan")
+    (d / "plan.cpp").write_text(SOURCE)
+    subprocess.run([cxx, "-O1", "-std=c++17", "-shared", "-fPIC", f"-I{CSRC}", str(d / "plan.cpp"), "-o",
+                    str(d / "plan.so")], check=True)
+    lib = ctypes.CDLL(str(d / "plan.so"))
+    lib.page.restype = ctypes.c_longlong
+    lib.page.argtypes = [ctypes.c_longlong] * 2
+    lib.seq.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]
+    lib.per_item.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
+    return lib
+
+
+def seq(lib, *given, tokens=100, indices=50, ps=16):
+    a, out = (ctypes.c_int * 5)(*given), (ctypes.c_int * 5)()
+    bad = lib.seq(a, tokens, indices, ps, out)
+    return bool(bad), list(out)
+
+
+def test_requests_inside_the_arrays(lib):
+    assert seq(lib, 0, 4, 0, 3, 7) == (False, [0, 4, 0, 3, 39])
+    assert seq(lib, 96, 100, 49, 50, 16) == (False, [96, 4, 49, 1, 16])
+    assert seq(lib, 5, 5, 7, 7, 0) == (False, [5, 0, 7, 0, 0])
+    assert seq(lib, 5, 6, 7, 8, 0) == (False, [5, 1, 7, 1, 0])
+
+
+@pytest.mark.parametrize("given,cut", [
+    ((-1, 4, 0, 3, 7), [0, 0, 0, 3, 39]), ((5, 4, 0, 3, 7), [0, 0, 0, 3, 39]), ((0, 101, 0, 3, 7), [0, 0, 0, 3, 39]),
+    ((0, 4, -1, 3, 7), [0, 4, 0, 0, 0]), ((0, 4, 3, 2, 7), [0, 4, 0, 0, 0]), ((0, 4, 0, 51, 7), [0, 4, 0, 0, 0]),
+    ((0, 4, 0, 3, 17), [0, 4, 0, 3, 48]), ((0, 4, 0, 3, -2), [0, 4, 0, 3, 32]),
+    ((-2 ** 31, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1), [0, 0, 0, 0, 0])])
+def test_broken_offsets_leave_nothing_outside(lib, given, cut):
+    assert seq(lib, *given) == (True, cut)
+
+
+def test_page_ids(lib):
+    assert [lib.page(i, 5) for i in (0, 4, -1, -5, 5, -6, 2 ** 31 - 1, -2 ** 31)] == [0, 4, 4, 0, -1, -1, -1, -1]
+    assert lib.page(0, 0) == -1
+
+
+def visible(p, j, window, sinks):
+    return j <= p and (window == 0 or p - j < window or j < sinks)
+
+
+def key_tiles(lib, *args):
+    out = (ctypes.c_int * 4096)()
+    n = lib.tiles(*args, out)
+    return list(out[:n])
+
+
+def test_key_tiles_hold_every_visible_key_once(lib):
+    rng = random.Random(1)
+    for _ in range(3000):
+        tile = rng.choice([32, 64])
+        kvlen = rng.choice([0, 1, rng.randint(1, 900)])
+        last = rng.randint(-3, max(kvlen - 1, 0))
+        first = last - rng.choice([0, 0, 3, rng.randint(0, 200)])
+        window = rng.choice([0, 1, rng.randint(1, 300), 2 ** 31 - 1])
+        sinks = rng.choice([0, 1, 4, rng.randint(0, 200), 2 ** 31 - 1])
+        got = key_tiles(lib, first, last, kvlen, window, sinks, tile)
+        assert got == sorted(set(got)) and all(0 <= t * tile < max(kvlen, 1) for t in got)
+        rows = range(first, last + 1)
+        need = {j // tile for j in range(kvlen) if any(visible(p, j, window, sinks) for p in (rows if len(rows) < 40 else (
+            first, last, *rng.sample(list(rows), 20))))}
+        assert need <= set(got), (first, last, kvlen, window, sinks, tile)
+        if last < 0 or kvlen == 0:
+            assert got == []
+    # a window keeps a long cache's walk short, and the largest values do not overflow
+    assert key_tiles(lib, 100000, 100000, 100001, 64, 4, 32) == [0, 3123, 3124, 3125]
+    assert key_tiles(lib, 2 ** 31 - 2, 2 ** 31 - 2, 2 ** 31 - 1, 1, 0, 64) == [(2 ** 31 - 2) // 64]
+
+
+def test_items_cover_every_block(lib):
+    """A block's key tiles never exceed what its items were counted for, and items of all
+    requests stay within the grid's bound."""
+    rng = random.Random(2)
+    for _ in range(400):
+        bm, tile = rng.choice([(16, 32), (16, 64), (64, 64), (128, 64)])
+        group = rng.choice([1, 2, 3, 4, 5, 8, 16, 71])
+        window, sinks = rng.choice([0, rng.randint(1, 300)]), rng.choice([0, 4, rng.randint(0, 130)])
+        requests = []
+        for _ in range(rng.randint(1, 6)):
+            kvlen = rng.randint(0, 700)
+            requests.append((rng.randint(0, min(kvlen + 2, 90)), kvlen))
+        total, plans = 0, []
+        for qlen, kvlen in requests:
+            blocks = ctypes.c_int()
+            tiles = lib.split(qlen, kvlen, group, bm, window, sinks, tile, ctypes.byref(blocks))
+            assert blocks.value == -(-qlen * group // bm)
+            for b in range(blocks.value):
+                r0, r1 = b * bm, min((b + 1) * bm, qlen * group) - 1
+                base = kvlen - qlen
+                assert len(key_tiles(lib, base + r0 // group, base + r1 // group, kvlen, window, sinks, tile)) <= tiles
+            total += blocks.value * tiles
+            plans.append((blocks.value, tiles))
+        target, least = rng.randint(1, 40), rng.choice([1, 2, 4])
+        per = lib.per_item(total, target, least)
+        items = sum(b * lib.chunks(b, t, per) for b, t in plans)
+        assert per >= least and items <= target + sum(b for b, _ in plans)
+        assert all(lib.chunks(b, t, per) * per >= t for b, t in plans)
+        rows = sum(q for q, _ in requests) * group
+        assert sum(b for b, _ in plans) <= min(rows, rows // bm + len(requests))
+    assert lib.chunks(1, 0, 4) == 1 and lib.chunks(1, 2 ** 31 - 1, 2 ** 31 - 1) == 1
+    assert lib.per_item(2 ** 60, 1, 2) == 0x3fffffff
