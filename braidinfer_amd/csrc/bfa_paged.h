@@ -108,4 +108,10 @@ BFA_HD int32_t paged_per_item(int64_t total, int32_t target, int32_t least) {
   return per < least ? least : static_cast<int32_t>(per > 0x3fffffff ? 0x3fffffff : per);
 }
 
+// Key tiles of each of a block's `chunks` items, so that they are alike: with `per`
+// tiles to the first and what is left to the last, the last would often be short.
+BFA_HD int32_t paged_even(int32_t tiles, int32_t chunks) {
+  return chunks > 1 ? tiles / chunks + (tiles % chunks != 0) : tiles;
+}
+
 }  // namespace bfa

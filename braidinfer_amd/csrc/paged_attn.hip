@@ -28,6 +28,8 @@
 // the chip, and a captured graph follows the lengths of each replay.
 #include <limits.h>
 
+#include <cmath>
+
 #include <type_traits>
 
 #include "bfa_device.h"
@@ -61,7 +63,8 @@ struct PagedArgs {
   int64_t tokens;
   uint32_t hq, hkv;
   FastDiv group, ps, heads;       // Hq / Hkv, page size, Hkv
-  float sl2, oscale;              // scale x log2(e), factor of the output
+  float sl2, oscale;              // |scale| x log2(e) (1 for a scale of 0), factor of the output
+  uint32_t qand, qxor;            // on pairs of query values: zero them, turn their signs
   int32_t window, sinks;
   uint16_t* out;                  // [tokens, Hq * D], row stride out_st
   int64_t out_st;
@@ -122,9 +125,14 @@ __device__ __forceinline__ bool pa_nonfinite(uint32_t w) {
   constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
+// zeros in place of infinities and NaN; whether there were any
 template <bool BF16>
-__device__ __forceinline__ bool pa_nonfinite(const uint4& v) {
-  return pa_nonfinite<BF16>(v.x) || pa_nonfinite<BF16>(v.y) || pa_nonfinite<BF16>(v.z) || pa_nonfinite<BF16>(v.w);
+__device__ __forceinline__ bool pa_make_finite(uint4& v) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  if (!(pa_nonfinite<BF16>(v.x) || pa_nonfinite<BF16>(v.y) || pa_nonfinite<BF16>(v.z) || pa_nonfinite<BF16>(v.w))) return false;
+  auto fix = [](uint32_t w) { return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u); };
+  v = make_uint4(fix(v.x), fix(v.y), fix(v.z), fix(v.w));
+  return true;
 }
 
 // word j of a quarter row of codes (8 or 16 bytes)
@@ -166,13 +174,19 @@ __device__ __forceinline__ uint4 v_fragment(const uint4* tile, int key0, int jd,
 }
 
 // Softmax and O^T += V^T P^T of one tile of 16 KC keys for RB blocks of 16 rows;
-// sc: the masked, scaled (base 2) scores of keys 16 c + 4 (lane / 16) + i.
-// `careful`: V holds an infinity or NaN and not every row sees every key, so
-// that a product with a weight of 0 must not happen.
+// sc: the masked scores of keys 16 c + 4 (lane / 16) + i, not yet times `sl2` (scale x
+// log2 e, not negative).  With the row's reference m, the largest score times sl2,
+// rounded, a weight is 2^(s sl2 - m): one multiply-add and one v_exp.  m's rounding error
+// is the same in every weight and in the sum and goes out with the division; from 2^16
+// on, where it could carry a weight past the type, the product is rounded first, as m's
+// was.  m follows a larger score only when that is more than LAG above it: weights then
+// reach 2^LAG, which fp32 sums and 16-bit weights do not mind, and most tiles after a
+// row's first few leave the accumulators alone.
 template <bool BF16, int D, int KC, int RB>
-__device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float (&m)[RB], float (&l)[RB],
-                                       pa_f32x4_t (&o)[RB][D / 16], const uint4* vt, int lane, bool careful) {
+__device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float sl2, float (&m)[RB], float (&l)[RB],
+                                       pa_f32x4_t (&o)[RB][D / 16], const uint4* vt, int lane) {
   constexpr int OJ = D / 16;
+  constexpr float LAG = 6.f;
   uint4 pf[RB][KC / 2];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -181,8 +195,8 @@ __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float (&m)[RB],
     for (int c = 0; c < KC; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[rb][c][i]);
-    mx = lanes4_max(mx);
-    if (__any(mx > m[rb])) {
+    mx = lanes4_max(mx) * sl2;
+    if (__any(mx - m[rb] > LAG)) {
       const float top = fmaxf(m[rb], mx);
       const float alpha = __builtin_amdgcn_exp2f(m[rb] - (top == -INFINITY ? 0.f : top));
       m[rb] = top;
@@ -192,13 +206,21 @@ __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float (&m)[RB],
     }
     const float ref = m[rb] == -INFINITY ? 0.f : m[rb];
     float sum = 0.f;
+    if (__any(fabsf(ref) >= 65536.f)) {
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[rb][c][i] = __builtin_amdgcn_exp2f(sc[rb][c][i] * sl2 - ref);
+    } else {
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[rb][c][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][c][i], sl2, -ref));
+    }
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[rb][c][i] = __builtin_amdgcn_exp2f(sc[rb][c][i] - ref);
-        sum += sc[rb][c][i];
-      }
+      for (int i = 0; i < 4; ++i) sum += sc[rb][c][i];
     l[rb] += sum;
 #pragma unroll
     for (int h = 0; h < KC / 2; ++h)
@@ -207,62 +229,35 @@ __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float (&m)[RB],
                              pa_pack<BF16>(sc[rb][2 * h + 1][0], sc[rb][2 * h + 1][1]),
                              pa_pack<BF16>(sc[rb][2 * h + 1][2], sc[rb][2 * h + 1][3]));
   }
-  if (!careful) {
 #pragma unroll
-    for (int h = 0; h < KC / 2; ++h)
+  for (int h = 0; h < KC / 2; ++h)
 #pragma unroll
-      for (int j = 0; j < OJ; ++j) {
-        const uint4 vf = v_fragment<D>(vt, 32 * h, j, lane);
+    for (int j = 0; j < OJ; ++j) {
+      const uint4 vf = v_fragment<D>(vt, 32 * h, j, lane);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) o[rb][j] = pa_mfma<BF16>(vf, pf[rb][h], o[rb][j]);
-      }
-    return;
-  }
-  // key by key, a lane's columns 16 j + 4 (lane / 16) + i of its row
-  const uint16_t* v16 = reinterpret_cast<const uint16_t*>(vt);
-  for (int g = 0; g < 4; ++g) {
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 16 * c + 4 * g + i;
-        float p[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) p[rb] = __shfl(sc[rb][c][i], (lane & 15) + 16 * g);
-#pragma unroll
-        for (int j = 0; j < OJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 16 * j + 4 * (lane >> 4) + e;
-            const float v = Elem<BF16 ? BFA_DTYPE_BF16 : BFA_DTYPE_F16>::to_f32(
-                v16[(key * (D / 8) + v_slot<D>(key, d >> 3)) * 8 + (d & 7)]);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-              if (p[rb] != 0.f) o[rb][j][e] += p[rb] * v;
-          }
-      }
-  }
+      for (int rb = 0; rb < RB; ++rb) o[rb][j] = pa_mfma<BF16>(vf, pf[rb][h], o[rb][j]);
+    }
 }
 
-// Scores times the scale; where `edge`, those of keys that a row does not see -inf
-// whatever they were.  hi: the row's position, lo: the first key of its window.
+// Scores of keys that a row does not see, or that do not exist, to -inf whatever they
+// were.  hi: the row's position, lo: the first key of its window.
 template <int KC, int RB>
-__device__ __forceinline__ void weigh(pa_f32x4_t (&sc)[RB][KC], float sl2, bool edge, int key0,
-                                      const int32_t (&hi)[RB], const int32_t (&lo)[RB], int32_t sinks, int lane) {
+__device__ __forceinline__ void hide(pa_f32x4_t (&sc)[RB][KC], uint64_t exists, int key0, const int32_t (&hi)[RB],
+                                     const int32_t (&lo)[RB], int32_t sinks, int lane) {
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-    for (int c = 0; c < KC; ++c) sc[rb][c] *= sl2;
-  if (!edge) return;
-#pragma unroll
-  for (int c = 0; c < KC; ++c)
+  for (int c = 0; c < KC; ++c) {
+    const uint32_t there = static_cast<uint32_t>(exists >> (16 * c)) >> (4 * (lane >> 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t key = key0 + 16 * c + 4 * (lane >> 4) + i;
+      const int32_t gone = ((there >> i) & 1) - 1, in = (key - sinks) >> 31;  // all ones: no such key; a sink
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        if (key > hi[rb] || (key < lo[rb] && key >= sinks)) sc[rb][c][i] = -INFINITY;
+      for (int rb = 0; rb < RB; ++rb) {
+        const int32_t hidden = gone | ((hi[rb] - key) >> 31) | (((key - lo[rb]) >> 31) & ~in);
+        sc[rb][c][i] = hidden < 0 ? -INFINITY : sc[rb][c][i];
+      }
     }
+  }
 }
 
 // first key of the window of a row at position p
@@ -281,7 +276,7 @@ __device__ __forceinline__ bool tile_edge(int32_t key0, int n, int32_t first, in
 // ------------------------------------------------------------------- items
 struct Item {
   PagedSeq s;
-  int32_t block, chunk, chunks, per, index;
+  int32_t block, chunk, chunks, index;
   bool live;
 };
 
@@ -334,7 +329,6 @@ __device__ __forceinline__ Item locate(const PagedArgs& a, int32_t x, bool write
     per = paged_per_item(total, a.target, a.least);
   }
   Item it{};
-  it.per = per;
   int32_t items = 0, blocks = 0;  // of the requests before
   for (int32_t b = lane;; b += 64) {
     if (b != lane) {
@@ -395,6 +389,12 @@ __device__ __forceinline__ Rows block_rows(const PagedArgs& a, const Item& it) {
   return r;
 }
 
+// 8 query values, with the scale's sign
+__device__ __forceinline__ uint4 query_words(const PagedArgs& a, const uint16_t* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  return make_uint4((v.x & a.qand) ^ a.qxor, (v.y & a.qand) ^ a.qxor, (v.z & a.qand) ^ a.qxor, (v.w & a.qand) ^ a.qxor);
+}
+
 // Address of a key: offsets of its row in the cache (16-byte units) and, in the
 // 4-bit cache, of its scales; ok: the key exists.
 struct KeyRow {
@@ -420,10 +420,101 @@ __device__ __forceinline__ KeyRow key_row(const PagedArgs& a, const PagedSeq& s,
   }
   return r;
 }
+// The rows of a key tile.  P16 (the page size is a multiple of 16): 16 keys from a
+// multiple of 16 lie on one page, so a lane resolves such a group (lane c group c), and
+// a load's address is the group's, in scalar registers, and an offset that the lane
+// keeps; otherwise a lane resolves a key, and loads take their rows' offsets from it.
+// (The 4-bit decode form is bound by the instructions it issues: TIME_P16.)
+template <bool FP4, bool P16, int KT>
+struct KeyTile {
+  KeyRow kr;
+  uint64_t exists;  // of the tile's keys
+
+  static constexpr uint64_t all() { return KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT & 63)) - 1; }
+  // the page list's entry that this lane resolves; asked for a tile ahead of its use
+  static __device__ __forceinline__ int32_t entry(const PagedArgs& a, const PagedSeq& s, int32_t key0, int lane) {
+    return key_entry(a, s, key0 + (P16 ? 16 * (lane & (KT / 16 - 1)) : lane & (KT - 1)));
+  }
+  __device__ __forceinline__ KeyTile(const PagedArgs& a, const PagedSeq& s, int32_t key0, int32_t id, int lane) {
+    if constexpr (P16) {
+      const int32_t key = key0 + 16 * (lane & (KT / 16 - 1));
+      kr = key_row<FP4>(a, s, key, id);
+      const uint64_t groups = __ballot(kr.ok || key >= s.kvlen);
+      exists = all();
+      if ((groups & ((1u << (KT / 16)) - 1)) != (1u << (KT / 16)) - 1) {
+#pragma unroll
+        for (int c = 0; c < KT / 16; ++c)
+          if (!((groups >> c) & 1)) exists &= ~(uint64_t{0xffff} << (16 * c));
+      }
+      const int32_t left = s.kvlen - key0;
+      if (left < KT) exists &= (uint64_t{1} << left) - 1;
+    } else {
+      kr = key_row<FP4>(a, s, key0 + (lane & (KT - 1)), id);
+      exists = __ballot(kr.ok) & all();
+    }
+  }
+  // offset (16-byte units) of row 16 c + base + sub, `sub` the lane's: of the group and
+  // the row's own in bytes, or of the row
+  __device__ __forceinline__ const uint8_t* row(const uint8_t* p, uint32_t stride, int c, int base, int sub, uint32_t part) const {
+    if constexpr (P16) {
+      const uint64_t g = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(kr.off), c))) * 16;
+      return p + g + static_cast<uint32_t>(base) * stride + (static_cast<uint32_t>(sub) * stride + part);
+    } else {
+      return p + static_cast<uint64_t>(__shfl(kr.off, 16 * c + base + sub)) * 16 + part;
+    }
+  }
+  __device__ __forceinline__ const uint8_t* scale(const uint8_t* p, uint32_t stride, int c, int sub, uint32_t part) const {
+    if constexpr (P16) {
+      return p + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(kr.soff), c)) + (static_cast<uint32_t>(sub) * stride + part);
+    } else {
+      return p + __shfl(kr.soff, 16 * c + sub) + part;
+    }
+  }
+};
 __device__ __forceinline__ uint4 zero_unless(bool ok, const uint4& v) {
   return make_uint4(ok ? v.x : 0u, ok ? v.y : 0u, ok ? v.z : 0u, ok ? v.w : 0u);
 }
 __device__ __forceinline__ uint2 zero_unless(bool ok, const uint2& v) { return make_uint2(ok ? v.x : 0u, ok ? v.y : 0u); }
+
+// What the tiles i0, i0 + step, .. of a block left out: infinities and NaN of V in tiles
+// that some row does not see all of, for the rows that see their key.  Runs only
+// where there are any, after the last tile.
+template <bool BF16, int D, bool FP4, int KT, int RB>
+__device__ __forceinline__ void poison(const PagedArgs& a, const PagedSeq& s, int32_t first, int32_t last, const KeyTiles& kt,
+                                       int32_t i0, int32_t i1, int32_t step, uint32_t h, const int32_t (&hi)[RB],
+                                       const int32_t (&lo)[RB], pa_f32x4_t (&o)[RB][D / 16], int lane) {
+  using E = Elem<BF16 ? BFA_DTYPE_BF16 : BFA_DTYPE_F16>;
+  const uint8_t* vbase = a.cache + h * a.c_sh + a.c_skv;
+  for (int32_t i = i0; i < i1; i += step) {
+    const int32_t key0 = kt.at(i) * KT;
+    if (!tile_edge(key0, KT, first, last, a.window, a.sinks)) continue;
+    for (int32_t key = key0; key < min(key0 + KT, s.kvlen); ++key) {
+      const KeyRow kr = key_row<FP4>(a, s, key, key_entry(a, s, key));
+      if (!kr.ok) continue;
+      const uint8_t* row = vbase + static_cast<uint64_t>(kr.off) * 16;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const int d = 16 * j + 4 * (lane >> 4);
+        uint2 w;
+        if constexpr (FP4) {
+          const float f = pa_scale<BF16>(a.scales[h * a.s_sh + a.s_skv + kr.soff + d / 32]);
+          const uint4 v = pa_from4<BF16>(*reinterpret_cast<const uint16_t*>(row + d / 2), f);
+          w = make_uint2(v.x, v.y);
+        } else {
+          w = *reinterpret_cast<const uint2*>(row + 2 * d);
+        }
+        if (!(pa_nonfinite<BF16>(w.x) || pa_nonfinite<BF16>(w.y))) continue;
+        const float v[4] = {E::to_f32(static_cast<uint16_t>(w.x & 0xffffu)), E::to_f32(static_cast<uint16_t>(w.x >> 16)),
+                            E::to_f32(static_cast<uint16_t>(w.y & 0xffffu)), E::to_f32(static_cast<uint16_t>(w.y >> 16))};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(fabsf(v[e]) < INFINITY) && key <= hi[rb] && (key >= lo[rb] || key < a.sinks)) o[rb][j][e] += v[e];
+      }
+    }
+  }
+}
 
 // ------------------------------------------------------------------ decode
 // Blocks of 16 rows, one kv head, 4 waves: wave w takes key tiles w, w + 4, ... of
@@ -432,9 +523,9 @@ __device__ __forceinline__ uint2 zero_unless(bool ok, const uint2& v) { return m
 // product reads; V goes through the wave's own LDS tile, for the transposing reads.
 // The next tile's rows are in flight during a tile's work, and the page ids of the
 // one after.  Bound by the cache's bytes.
-template <bool BF16, int D, bool FP4>
-__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
-  constexpr int KT = FP4 ? 64 : 32, KC = KT / 16;
+template <bool BF16, int D, bool FP4, bool P16>
+__global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(PagedArgs a) {
+  constexpr int KT = 32, KC = KT / 16;
   constexpr int GK = D / 8, QJ = D / 32, OJ = D / 16;
   constexpr int VN = FP4 ? KT / 16 : KT * GK / 64;  // V loads of a lane: a quarter row of codes, or a granule
   using Code = std::conditional_t<FP4 && D == 64, uint2, uint4>;  // a quarter row of codes, or a granule
@@ -448,8 +539,8 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
   if (!it.live) return;
   const Rows rows = block_rows<16>(a, it);
   const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
-  const int32_t i0 = it.chunks > 1 ? it.chunk * it.per : 0;
-  const int32_t i1 = it.chunks > 1 ? min(i0 + it.per, kt.count) : kt.count;
+  const int32_t per = paged_even(kt.count, it.chunks);
+  const int32_t i0 = min(it.chunk * per, kt.count), i1 = min(i0 + per, kt.count);
 
   // this lane's row: its query, as the B operand of S^T, and its position
   uint4 qf[QJ];
@@ -462,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
     // are its columns of the query)
 #pragma unroll
     for (int j = 0; j < QJ; ++j)
-      qf[j] = *reinterpret_cast<const uint4*>(qrow + (FP4 ? D / 4 * g4 + 8 * j : 32 * j + 8 * g4));
+      qf[j] = query_words(a, qrow + (FP4 ? D / 4 * g4 + 8 * j : 32 * j + 8 * g4));
     hi[0] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
     lo[0] = window_from(hi[0], a.window);
   }
@@ -474,64 +565,53 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
 
   const uint8_t* kbase = a.cache + h * a.c_sh;
   const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh : nullptr;
+  const uint32_t cstride = a.c_ss * 16;  // of the slots, in bytes
   struct Tile {
     uint4 k[FP4 ? 1 : KC][FP4 ? 1 : QJ];
     Code kc[FP4 ? KC : 1], v[VN];
     uint32_t ks[FP4 ? KC : 1], vs[FP4 ? VN : 1];
-    uint32_t ok;  // of the rows of v
   };
-  // lane l resolves key l % KT of a tile; its loads take the rows from there
-  auto entry = [&](int32_t i) { return key_entry(a, it.s, kt.at(min(i, kt.count - 1)) * KT + (lane & (KT - 1))); };
-  auto issue = [&](int32_t i, int32_t id) {
+  using Keys = KeyTile<FP4, P16, KT>;
+  auto entry = [&](int32_t i) { return Keys::entry(a, it.s, kt.at(min(i, kt.count - 1)) * KT, lane); };
+  auto issue = [&](const Keys& keys) {
     Tile t;
-    const KeyRow kr = key_row<FP4>(a, it.s, kt.at(i) * KT + (lane & (KT - 1)), id);
-    const uint64_t okay = __ballot(kr.ok);
-    t.ok = 0;
     if constexpr (FP4) {
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        const uint32_t off = __shfl(kr.off, 16 * c + (lane & 15)), soff = __shfl(kr.soff, 16 * c + (lane & 15));
-        t.kc[c] = *reinterpret_cast<const Code*>(kbase + static_cast<uint64_t>(off) * 16 + D / 8 * g4);
-        t.ks[c] = ksc[static_cast<uint64_t>(soff) + D / 4 * g4 / 32];
+        t.kc[c] = *reinterpret_cast<const Code*>(keys.row(kbase, cstride, c, 0, lane & 15, D / 8 * g4));
+        t.ks[c] = *keys.scale(ksc, a.s_ss, c, lane & 15, D / 4 * g4 / 32);
       }
 #pragma unroll
       for (int i = 0; i < VN; ++i) {
-        const int r = 16 * i + (lane >> 2);
-        const uint32_t off = __shfl(kr.off, r), soff = __shfl(kr.soff, r);
-        t.v[i] = *reinterpret_cast<const Code*>(kbase + a.c_skv + static_cast<uint64_t>(off) * 16 + D / 8 * (lane & 3));
-        t.vs[i] = ksc[a.s_skv + static_cast<uint64_t>(soff) + D / 4 * (lane & 3) / 32];
-        t.ok |= static_cast<uint32_t>((okay >> r) & 1) << i;
+        t.v[i] = *reinterpret_cast<const Code*>(keys.row(kbase + a.c_skv, cstride, i, 0, lane >> 2, D / 8 * (lane & 3)));
+        t.vs[i] = *keys.scale(ksc + a.s_skv, a.s_ss, i, lane >> 2, D / 4 * (lane & 3) / 32);
       }
     } else {
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        const uint32_t off = __shfl(kr.off, 16 * c + (lane & 15));
-        const uint8_t* row = kbase + static_cast<uint64_t>(off) * 16 + 16 * g4;
+        const uint8_t* row = keys.row(kbase, cstride, c, 0, lane & 15, 16 * g4);
 #pragma unroll
         for (int j = 0; j < QJ; ++j) t.k[c][j] = *reinterpret_cast<const uint4*>(row + 64 * j);
       }
 #pragma unroll
-      for (int i = 0; i < VN; ++i) {
-        const int r = 64 / GK * i + lane / GK;
-        const uint32_t off = __shfl(kr.off, r);
-        t.v[i] = *reinterpret_cast<const uint4*>(kbase + a.c_skv + static_cast<uint64_t>(off) * 16 + 16 * (lane % GK));
-        t.ok |= static_cast<uint32_t>((okay >> r) & 1) << i;
-      }
+      for (int i = 0; i < VN; ++i)
+        t.v[i] = *reinterpret_cast<const uint4*>(
+            keys.row(kbase + a.c_skv, cstride, 64 / GK * i / 16, 64 / GK * i % 16, lane / GK, 16 * (lane % GK)));
     }
     return t;
   };
 
   uint4* vt = vbuf[wid];
+  bool odd = false;
   int32_t i = i0 + wid;
   if (i < i1) {
-    Tile cur = issue(i, entry(i));
-    int32_t id = entry(i + 4);
+    int32_t id = entry(i);
     for (; i < i1; i += 4) {
       const int32_t key0 = kt.at(i) * KT;
       const bool edge = tile_edge(key0, KT, rows.first, rows.last, a.window, a.sinks);
-      const int32_t id2 = entry(i + 8);
-      Tile nxt;
-      if (i + 4 < i1) nxt = issue(i + 4, id);
+      const int32_t id2 = entry(i + 4);
+      const Keys keys(a, it.s, key0, id, lane);
+      const Tile cur = issue(keys);
       id = id2;
       // S^T = K Q^T
       pa_f32x4_t sc[1][KC];
@@ -547,40 +627,47 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
             sc[0][c] = pa_mfma<BF16>(cur.k[c][j], qf[j], sc[0][c]);
           }
         }
-      weigh<KC, 1>(sc, a.sl2, edge, key0, hi, lo, a.sinks, lane);
-      // V -> LDS; rows that do not exist as zeros, since 0 x a NaN would poison the sum
-      bool odd = false;
+      const bool whole = keys.exists == Keys::all();
+      if (edge || !whole) hide<KC, 1>(sc, keys.exists, key0, hi, lo, a.sinks, lane);
+      // V -> LDS; rows that do not exist as zeros, since 0 x a NaN would poison the sum,
+      // and likewise what is not finite in a tile that some row does not see all of
       __builtin_amdgcn_wave_barrier();
       if constexpr (FP4) {
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int r = 16 * i + (lane >> 2);
-          const bool ok = (cur.ok >> i) & 1;
-          const Code c = zero_unless(ok, cur.v[i]);
-          const float s = ok ? pa_scale<BF16>(cur.vs[i]) : 1.f;
+          Code c = cur.v[i];
+          float s = pa_scale<BF16>(cur.vs[i]);
+          if (!whole) {
+            const bool ok = (keys.exists >> r) & 1;
+            c = zero_unless(ok, c);
+            s = ok ? s : 1.f;
+          }
 #pragma unroll
           for (int k = 0; k < QJ; ++k) {
-            const uint4 x = pa_from4<BF16>(pa_word(c, k), s);
+            uint4 x = pa_from4<BF16>(pa_word(c, k), s);
+            if (edge) odd |= pa_make_finite<BF16>(x);
             vt[r * GK + v_slot<D>(r, QJ * (lane & 3) + k)] = x;
-            if (edge && pa_nonfinite<BF16>(x)) odd = true;
           }
         }
       } else {
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int r = 64 / GK * i + lane / GK;
-          const uint4 x = zero_unless((cur.ok >> i) & 1, cur.v[i]);
+          uint4 x = cur.v[i];
+          if (!whole) x = zero_unless((keys.exists >> r) & 1, x);
+          if (edge) odd |= pa_make_finite<BF16>(x);
           vt[r * GK + v_slot<D>(r, lane % GK)] = x;
-          if (edge && pa_nonfinite<BF16>(x)) odd = true;
         }
       }
       asm volatile("" ::: "memory");  // (one wave's LDS accesses happen in order)
       __builtin_amdgcn_wave_barrier();
-      attend<BF16, D, KC, 1>(sc, m, l, o, vt, lane, __any(odd));
+      attend<BF16, D, KC, 1>(sc, a.sl2, m, l, o, vt, lane);
       asm volatile("" ::: "memory");
-      cur = nxt;
     }
   }
+
+  if (__any(odd)) poison<BF16, D, FP4, KT, 1>(a, it.s, rows.first, rows.last, kt, i0 + wid, i1, 4, h, hi, lo, o, lane);
 
   // the four waves' states meet: granule G (4 columns) of row r at slot G ^ r
   l[0] = lanes4_sum(l[0]);
@@ -638,7 +725,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedArgs a) {
 // tiles of 64, which all of them load into the LDS (two tiles: the next one's rows
 // are in flight in registers during a tile's matrix work).  Bound by the matrix
 // cores and the LDS that feeds them.
-template <bool BF16, int D, bool FP4, int RB>
+template <bool BF16, int D, bool FP4, bool P16, int RB>
 __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   constexpr int KT = 64, KC = 4, BM = 64 * RB;
   constexpr int GK = D / 8, QJ = D / 32, OJ = D / 16;
@@ -656,8 +743,8 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   if (!it.live) return;
   const Rows rows = block_rows<BM>(a, it);
   const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
-  const int32_t i0 = it.chunks > 1 ? it.chunk * it.per : 0;
-  const int32_t i1 = it.chunks > 1 ? min(i0 + it.per, kt.count) : kt.count;
+  const int32_t per = paged_even(kt.count, it.chunks);
+  const int32_t i0 = min(it.chunk * per, kt.count), i1 = min(i0 + per, kt.count);
 
   uint4 qf[RB][QJ];
   int32_t hi[RB], lo[RB];
@@ -667,7 +754,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
     const uint16_t* qrow =
         a.q + (it.s.q0 + static_cast<int64_t>(t)) * a.q_st + (h * a.group.d + (r - t * a.group.d)) * a.q_sh;
 #pragma unroll
-    for (int j = 0; j < QJ; ++j) qf[rb][j] = *reinterpret_cast<const uint4*>(qrow + 32 * j + 8 * g4);
+    for (int j = 0; j < QJ; ++j) qf[rb][j] = query_words(a, qrow + 32 * j + 8 * g4);
     hi[rb] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
     lo[rb] = window_from(hi[rb], a.window);
   }
@@ -687,92 +774,88 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
     for (int j = 0; j < OJ; ++j) o[rb][j] = pa_f32x4_t{};
   }
 
-  // staging: row of load n, and this thread's part of a row
-  auto row_of = [&](int n) { return FP4 ? tid >> 2 : tid / GK + 256 / GK * n; };
-  const int part = FP4 ? tid & 3 : tid % GK;
-  const uint8_t* kbase = a.cache + h * a.c_sh + (FP4 ? D / 8 : 16) * part;
-  const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh + D / 4 * part / 32 : nullptr;
+  // staging: load n takes row 16 c + base + sub of the tile, a wave the rows of one group
+  constexpr int WR = FP4 ? 16 : 64 / GK;  // rows of a wave in one load
+  const int sub = FP4 ? lane >> 2 : lane / GK, part = FP4 ? lane & 3 : lane % GK;
+  auto row0_of = [&](int n) { return WR * wid + 4 * WR * n; };
+  const uint8_t* kbase = a.cache + h * a.c_sh;
+  const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh : nullptr;
+  const uint32_t cstride = a.c_ss * 16;
+  using Keys = KeyTile<FP4, P16, KT>;
   struct Tile {
     Code k[NL], v[NL];
     uint32_t ks, vs;
-    bool ok[NL];
   };
-  struct Ids {
-    int32_t id[NL];
-  };
-  auto entries = [&](int32_t i) {
-    Ids e;
-    const int32_t key0 = kt.at(min(i, kt.count - 1)) * KT;
-#pragma unroll
-    for (int n = 0; n < NL; ++n) e.id[n] = key_entry(a, it.s, key0 + row_of(n));
-    return e;
-  };
-  auto issue = [&](int32_t i, const Ids& e) {
+  auto entry = [&](int32_t i) { return Keys::entry(a, it.s, kt.at(min(i, kt.count - 1)) * KT, lane); };
+  auto issue = [&](const Keys& keys) {
     Tile t;
-    const int32_t key0 = kt.at(i) * KT;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      const KeyRow kr = key_row<FP4>(a, it.s, key0 + row_of(n), e.id[n]);
-      const uint8_t* p = kbase + static_cast<uint64_t>(kr.off) * 16;
+      const int r0 = row0_of(n);
+      const uint8_t* p = keys.row(kbase, cstride, r0 / 16, r0 % 16, sub, (FP4 ? D / 8 : 16) * part);
       t.k[n] = *reinterpret_cast<const Code*>(p);
       t.v[n] = *reinterpret_cast<const Code*>(p + a.c_skv);
       if constexpr (FP4) {
-        t.ks = ksc[kr.soff];
-        t.vs = ksc[a.s_skv + kr.soff];
+        const uint8_t* f = keys.scale(ksc, a.s_ss, r0 / 16, sub, D / 4 * part / 32);
+        t.ks = *f;
+        t.vs = f[a.s_skv];
       }
-      t.ok[n] = kr.ok;
     }
     return t;
   };
-  // a tile into the LDS, rows that do not exist as zeros; whether its V holds an
-  // infinity or NaN, asked where some row does not see all of it
-  auto store = [&](const Tile& t, int b, bool edge) {
-    bool odd = false;
+  // a tile into the LDS, rows that do not exist as zeros, and so what is not finite in
+  // a V tile that some row does not see all of
+  bool odd = false;
+  auto store = [&](const Tile& t, int b, uint64_t exists, bool edge) {
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      const int r = row_of(n);
-      const Code kc = zero_unless(t.ok[n], t.k[n]), vc = zero_unless(t.ok[n], t.v[n]);
+      const int r = row0_of(n) + sub;
+      Code kc = t.k[n], vc = t.v[n];
+      float fk = 1.f, fv = 1.f;
+      if constexpr (FP4) fk = pa_scale<BF16>(t.ks), fv = pa_scale<BF16>(t.vs);
+      if (exists != Keys::all()) {
+        const bool ok = (exists >> r) & 1;
+        kc = zero_unless(ok, kc), vc = zero_unless(ok, vc);
+        fk = ok ? fk : 1.f, fv = ok ? fv : 1.f;
+      }
       if constexpr (FP4) {
-        const float fk = t.ok[n] ? pa_scale<BF16>(t.ks) : 1.f, fv = t.ok[n] ? pa_scale<BF16>(t.vs) : 1.f;
 #pragma unroll
         for (int k = 0; k < QJ; ++k) {
-          const uint4 xv = pa_from4<BF16>(pa_word(vc, k), fv);
+          uint4 xv = pa_from4<BF16>(pa_word(vc, k), fv);
+          if (edge) odd |= pa_make_finite<BF16>(xv);
           kbuf[b][r * GK + k_slot<D>(r, QJ * part + k)] = pa_from4<BF16>(pa_word(kc, k), fk);
           vbuf[b][r * GK + v_slot<D>(r, QJ * part + k)] = xv;
-          if (edge && pa_nonfinite<BF16>(xv)) odd = true;
         }
       } else {
+        if (edge) odd |= pa_make_finite<BF16>(vc);
         kbuf[b][r * GK + k_slot<D>(r, part)] = kc;
         vbuf[b][r * GK + v_slot<D>(r, part)] = vc;
-        if (edge && pa_nonfinite<BF16>(vc)) odd = true;
       }
     }
-    return odd;
   };
   auto wg_edge = [&](int32_t i) {
     return tile_edge(kt.at(i) * KT, KT, rows.first, rows.last, a.window, a.sinks);
   };
-  // every wave's part of a tile is in the LDS, and every wave is done with the other
-  auto meet = [&](bool edge, bool odd) {
-    if (edge) return __syncthreads_or(odd) != 0;
-    __syncthreads();
-    return false;
-  };
-
   if (i0 < i1) {
-    Ids id = entries(i0);
-    Tile cur = issue(i0, id);
-    id = entries(i0 + 1);
-    bool careful;
+    uint64_t exists, ahead;
+    Tile cur;
     {
-      const bool e = wg_edge(i0);
-      careful = meet(e, store(cur, 0, e));
+      const Keys keys(a, it.s, kt.at(i0) * KT, entry(i0), lane);
+      cur = issue(keys);
+      exists = ahead = keys.exists;
     }
+    int32_t id = entry(i0 + 1);
+    store(cur, 0, exists, wg_edge(i0));
+    __syncthreads();
     for (int32_t i = i0; i < i1; ++i) {
       const int b = (i - i0) & 1;
       const bool more = i + 1 < i1;
-      const Ids id2 = entries(i + 2);
-      if (more) cur = issue(i + 1, id);
+      const int32_t id2 = entry(i + 2);
+      if (more) {
+        const Keys keys(a, it.s, kt.at(i + 1) * KT, id, lane);
+        cur = issue(keys);
+        ahead = keys.exists;
+      }
       id = id2;
       const int32_t key0 = kt.at(i) * KT;
       // (a wave skips a tile that none of its rows sees)
@@ -791,14 +874,17 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) sc[rb][c] = pa_mfma<BF16>(kf, qf[rb][j], sc[rb][c]);
           }
-        weigh<KC, RB>(sc, a.sl2, tile_edge(key0, KT, wfirst, wlast, a.window, a.sinks), key0, hi, lo, a.sinks, lane);
-        attend<BF16, D, KC, RB>(sc, m, l, o, vbuf[b], lane, careful);
+        if (tile_edge(key0, KT, wfirst, wlast, a.window, a.sinks) || exists != Keys::all())
+          hide<KC, RB>(sc, exists, key0, hi, lo, a.sinks, lane);
+        attend<BF16, D, KC, RB>(sc, a.sl2, m, l, o, vbuf[b], lane);
       }
       if (more) {
-        const bool e = wg_edge(i + 1);
-        careful = meet(e, store(cur, b ^ 1, e));
+        store(cur, b ^ 1, ahead, wg_edge(i + 1));
+        exists = ahead;
+        __syncthreads();  // the tile is whole, and every wave is done with the other
       }
     }
+    if (__syncthreads_or(odd)) poison<BF16, D, FP4, KT, RB>(a, it.s, rows.first, rows.last, kt, i0, i1, 1, h, hi, lo, o, lane);
   }
 
 #pragma unroll
@@ -826,18 +912,24 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 }
 
 // ------------------------------------------------------------------- merge
-// Joins the items of each block that has several: a group of D / 4 lanes takes 4
-// columns each of every (64 / (D / 4))-th item of a row, the groups of a wave meet
-// by lane swaps, in one order whatever runs first.
+// Joins the items of each block that has several: a wave takes a row, or up to 16
+// items of it at a time where there are more and the workgroup's four waves share the
+// row (30000 keys of one request: TIME_MERGE); D / 4 lanes have 4 columns each, the 64 /
+// (D / 4) groups of lanes every such item, and meet by lane exchanges, the waves in the
+// LDS, in one order whatever runs first.
 template <bool BF16, int D, int BM>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  constexpr int L = D / 4, NG = 64 / L, U = 8;
+  constexpr int L = D / 4, NG = 64 / L, U = 16 / NG;
+  __shared__ float4 wacc[4][L];
+  __shared__ float wsum[4];
   const uint32_t block = a.heads.div(blockIdx.x), h = blockIdx.x - block * a.hkv;
   const int4 line = a.table[block];
   const int32_t items = line.y, n = line.w;
   if (items <= 1) return;
-  const int lane = threadIdx.x & 63, sub = lane / L, col = lane % L;
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < n; r += 4 * gridDim.y) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, sub = lane / L, col = lane % L;
+  const bool wide = items > 16;
+  const int step_r = (wide ? 1 : 4) * gridDim.y;
+  for (int r = wide ? blockIdx.y : blockIdx.y * 4 + wid; r < n; r += step_r) {
     const int64_t slot0 = (static_cast<int64_t>(line.x) * a.hkv + h) * BM + r, step = static_cast<int64_t>(a.hkv) * BM;
     const float2* ml = reinterpret_cast<const float2*>(a.ml) + slot0;
     float mx = -INFINITY;
@@ -846,7 +938,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
     const float ref = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
     float4 acc = {};
-    for (int z0 = 0; z0 < items; z0 += NG * U) {
+    for (int z0 = wide ? 16 * wid : 0; z0 < items; z0 += wide ? 64 : 16) {
       float2 st[U];
       float4 v[U];
 #pragma unroll
@@ -869,7 +961,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
       acc.x += __shfl_xor(acc.x, d); acc.y += __shfl_xor(acc.y, d);
       acc.z += __shfl_xor(acc.z, d); acc.w += __shfl_xor(acc.w, d);
     }
-    if (sub) continue;
+    if (wide) {  // (the same for the whole workgroup)
+      if (sub == 0) wacc[wid][col] = acc;
+      if (lane == 0) wsum[wid] = sum;
+      __syncthreads();
+      sum = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+      const float4 p = wacc[0][col], q = wacc[1][col], s = wacc[2][col], t = wacc[3][col];
+      acc = make_float4(p.x + q.x + s.x + t.x, p.y + q.y + s.y + t.y, p.z + q.z + s.z + t.z, p.w + q.w + s.w + t.w);
+      __syncthreads();
+    }
+    if (sub || (wide && wid)) continue;
     const float inv = sum == 0.f ? 0.f : a.oscale / sum;
     const uint32_t rr = static_cast<uint32_t>(line.z) + r, t = a.group.div(rr);
     uint16_t* orow = a.out + static_cast<int64_t>(t) * a.out_st + (h * a.group.d + (rr - t * a.group.d)) * static_cast<int64_t>(D);
@@ -889,18 +990,25 @@ struct PagedPlan {
 // The form follows the rows of an average request, and the items the workgroups that
 // fill the chip; the lengths themselves stay on the device.
 static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int64_t hkv, int64_t d,
-                            int64_t num_indices, int64_t page_size, int64_t window, int64_t sinks, bool fp4) {
+                            int64_t num_indices, int64_t page_size, int64_t window, int64_t sinks) {
   PagedPlan p{};
   const int64_t rows = tokens * group;
   p.rb = rows <= 16 * num_seqs ? 0 : rows <= 64 * num_seqs ? 1 : 2;
+  const int forced = tuning(BFA_TUNE_PAGED_ROWS);  // planner override
+  if (forced == 16 || forced == 64 || forced == 128) p.rb = forced / 64;
   p.bm = p.rb == 0 ? 16 : 64 * p.rb;
-  const int64_t kt = p.rb == 0 && !fp4 ? 32 : 64;
+  const int64_t kt = p.rb == 0 ? 32 : 64;
   p.nblocks = static_cast<int32_t>(std::min(rows, rows / p.bm + num_seqs));
   p.least = p.rb == 0 ? 4 : 2;
-  p.target = static_cast<int32_t>(std::max<int64_t>(1, cdiv(p.rb == 0 ? 1024 : 512, hkv)));
-  int64_t most = cdiv(num_indices * page_size, kt);  // key tiles of a block
+  const int64_t all = cdiv(num_indices * page_size, kt) + num_seqs;  // key tiles of all requests
+  int64_t most = all;                                               // of a block
   if (window > 0) most = std::min(most, (window + p.bm / group + 2) / kt + 2 + sinks / kt + 1);
+  const int wanted = tuning(BFA_TUNE_PAGED_WG);  // planner override
+  int64_t wish = cdiv(wanted > 0 ? wanted : p.rb == 0 ? 2560 : 512, hkv);
+  if (wanted <= 0) wish = std::max<int64_t>(wish - p.nblocks, cdiv(wish, 4));
+  p.target = static_cast<int32_t>(std::max<int64_t>(1, std::min(wish, std::min(all, p.nblocks * most) / p.least)));
   p.split = most > p.least && (p.rb == 0 ? p.nblocks * hkv < 8192 : p.nblocks * hkv < 1024);
+  if (wanted >= 0) p.split = wanted > 0 && most > p.least;
   p.items = p.nblocks + (p.split ? p.target : 0);
   if (p.split) {
     const int64_t slots = static_cast<int64_t>(p.items) * hkv * p.bm;
@@ -942,7 +1050,7 @@ extern "C" int64_t bfa_paged_attention_workspace_size(int64_t tokens, int64_t nu
                    page_size) != BFA_OK)
     return 0;
   return paged_plan(tokens, num_seqs, num_q_heads / num_kv_heads, num_kv_heads, head_dim, num_indices, page_size, window,
-                    sinks, cache_dtype == BFA_DTYPE_FP4).total();
+                    sinks).total();
 }
 
 extern "C" int bfa_paged_attention(
@@ -982,7 +1090,7 @@ extern "C" int bfa_paged_attention(
   const int64_t win = window >= (int64_t{1} << 31) ? 0 : window;  // (wider than any cache: no window)
   const int64_t snk = std::min<int64_t>(sinks, (int64_t{1} << 31) - 1);
   const int64_t group = num_q_heads / num_kv_heads;
-  const PagedPlan p = paged_plan(num_tokens, num_seqs, group, num_kv_heads, head_dim, num_indices, page_size, win, snk, fp4);
+  const PagedPlan p = paged_plan(num_tokens, num_seqs, group, num_kv_heads, head_dim, num_indices, page_size, win, snk);
   BFA_REQUIRE(p.total() == 0 || (workspace && workspace_bytes >= p.total()), "%s: workspace too small", what);
 
   PagedArgs a{};
@@ -1005,7 +1113,9 @@ extern "C" int bfa_paged_attention(
   a.ps = FastDiv(static_cast<uint32_t>(page_size));
   a.heads = FastDiv(a.hkv);
   const float back = fp4 && dtype == BFA_DTYPE_F16 ? 16.f : 1.f;
-  a.sl2 = scale * 1.4426950408889634f * back;
+  a.sl2 = scale == 0.f ? 1.f : fabsf(scale * 1.4426950408889634f) * back;
+  a.qand = scale == 0.f ? 0u : 0xffffffffu;
+  a.qxor = scale < 0.f ? 0x80008000u : 0u;
   a.oscale = back;
   a.window = static_cast<int32_t>(win); a.sinks = static_cast<int32_t>(snk);
   a.out = static_cast<uint16_t*>(out); a.out_st = out_stride_token;
@@ -1017,24 +1127,27 @@ extern "C" int bfa_paged_attention(
   a.status = status;
   const hipStream_t s = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(p.items * num_kv_heads));
-  auto launch = [&](auto bf, auto dd, auto four) {
-    constexpr bool B = decltype(bf)::value, F = decltype(four)::value;
+  const bool p16 = page_size % 16 == 0 && stride_slot / unit < (int64_t{1} << 23) && scale_stride_slot < (int64_t{1} << 27);
+  auto launch = [&](auto bf, auto dd, auto four, auto by16) {
+    constexpr bool B = decltype(bf)::value, F = decltype(four)::value, P = decltype(by16)::value;
     constexpr int DD = decltype(dd)::value;
     const unsigned blocks = static_cast<unsigned>(p.nblocks * num_kv_heads);
     if (p.rb == 0) {
-      hipLaunchKernelGGL((paged_decode_kernel<B, DD, F>), grid, dim3(256), 0, s, a);
-      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 16>), dim3(blocks), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((paged_decode_kernel<B, DD, F, P>), grid, dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 16>), dim3(blocks, blocks < 512 ? 4 : 1), dim3(256), 0, s, a);
     } else if (p.rb == 1) {
-      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, 1>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, P, 1>), grid, dim3(256), 0, s, a);
       if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 64>), dim3(blocks, 4), dim3(256), 0, s, a);
     } else {
-      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, 2>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, P, 2>), grid, dim3(256), 0, s, a);
       if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 128>), dim3(blocks, 8), dim3(256), 0, s, a);
     }
   };
   auto with_d = [&](auto bf, auto four) {
-    if (head_dim == 64) launch(bf, std::integral_constant<int, 64>{}, four);
-    else launch(bf, std::integral_constant<int, 128>{}, four);
+    auto with_p = [&](auto dd) {
+      if (p16) launch(bf, dd, four, std::true_type{}); else launch(bf, dd, four, std::false_type{});
+    };
+    if (head_dim == 64) with_p(std::integral_constant<int, 64>{}); else with_p(std::integral_constant<int, 128>{});
   };
   if (dtype == BFA_DTYPE_BF16) {
     if (fp4) with_d(std::true_type{}, std::true_type{}); else with_d(std::true_type{}, std::false_type{});

@@ -13,7 +13,6 @@ whose page manager keeps a 16-bit cache (engine/page_manager.py:36-42).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
@@ -21,7 +20,6 @@ import torch
 from .. import _lib
 
 
-@dataclass
 class Fp4KVCache:
     """One layer of the cache, [pages, 2, kv heads, page slots, ...], K at index 0.
 
@@ -29,19 +27,22 @@ class Fp4KVCache:
     bits of byte i; scales: uint8 [..., head_dim / 32], 127 + the scale's exponent (255:
     the block reads as NaN)."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("codes", "scales", "num_pages", "num_kv_heads", "page_size", "head_dim", "strides")
 
-    def __post_init__(self):
-        c, s = self.codes, self.scales
-        if c.dtype != torch.uint8 or s.dtype != torch.uint8:
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales must be uint8")
-        if c.dim() != 5 or s.dim() != 5 or c.shape[1] != 2 or c.shape[:4] != s.shape[:4] or c.shape[4] != 16 * s.shape[4]:
-            raise ValueError(f"codes {tuple(c.shape)} and scales {tuple(s.shape)} must be "
+        c, s = codes.shape, scales.shape
+        if len(c) != 5 or len(s) != 5 or c[1] != 2 or c[:4] != s[:4] or c[4] != 16 * s[4]:
+            raise ValueError(f"codes {tuple(c)} and scales {tuple(s)} must be "
                              "[pages, 2, heads, slots, head_dim / 2] and [pages, 2, heads, slots, head_dim / 32]")
-        if c.stride(4) != 1 or s.stride(4) != 1:
-            if c.shape[4] and (c.stride(4) != 1 or s.shape[4] > 1):
-                raise ValueError("codes and scales must have unit stride along head_dim")
+        cs, ss = codes.stride(), scales.stride()
+        if (cs[4] != 1 and c[4] > 1) or (ss[4] != 1 and s[4] > 1):
+            raise ValueError("codes and scales must have unit stride along head_dim")
+        self.codes, self.scales = codes, scales
+        self.num_pages, _, self.num_kv_heads, self.page_size, half = c
+        self.head_dim = 2 * half
+        self.strides = cs[:4] + ss[:4]  # (page, K|V, head, slot) of the codes and of the scales, in bytes
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device=None) -> "Fp4KVCache":
@@ -54,53 +55,43 @@ class Fp4KVCache:
         return cls(torch.empty(*shape, head_dim // 2, dtype=torch.uint8, device=device),
                    torch.empty(*shape, head_dim // 32, dtype=torch.uint8, device=device))
 
-    @property
-    def num_pages(self) -> int:
-        return self.codes.shape[0]
 
-    @property
-    def num_kv_heads(self) -> int:
-        return self.codes.shape[2]
-
-    @property
-    def page_size(self) -> int:
-        return self.codes.shape[3]
-
-    @property
-    def head_dim(self) -> int:
-        return 2 * self.codes.shape[4]
+_INTS = {torch.int32: _lib.I32, torch.int64: _lib.I64}
+_FLOATS = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _ints(name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
+def _ints(name: str, t: torch.Tensor):
+    """(contiguous one-dimensional tensor, its dtype's code)"""
+    code = _INTS.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
     if t.dim() != 1:
         raise ValueError(f"{name} must be one-dimensional")
-    return t.contiguous()
+    return (t if t.is_contiguous() else t.contiguous()), code
 
 
 def _tokens(cache, kv_indices, kv_indptr, batch_indices, positions, num_tokens):
     """Checked token addressing: the tensors, which the call must keep, and their
     entry-point arguments."""
-    positions, kv_indices = _ints("positions", positions), _ints("kv_indices", kv_indices)
+    positions, pos_code = _ints("positions", positions)
+    kv_indices, idx_code = _ints("kv_indices", kv_indices)
     if positions.shape[0] != num_tokens:
         raise IndexError(f"{positions.shape[0]} positions for {num_tokens} tokens")
     if (kv_indptr is None) != (batch_indices is None):
         raise ValueError("kv_indptr and batch_indices go together")
+    batched = (None, None, 0, 0)
     if kv_indptr is not None:
-        batch_indices = _ints("batch_indices", batch_indices)
+        batch_indices, code = _ints("batch_indices", batch_indices)
         if batch_indices.shape[0] != num_tokens:
             raise IndexError(f"{batch_indices.shape[0]} batch indices for {num_tokens} tokens")
         if kv_indptr.dtype != torch.int32 or kv_indptr.dim() != 1 or kv_indptr.shape[0] < 1:
             raise TypeError("kv_indptr must be a one-dimensional int32 tensor")
-        kv_indptr = kv_indptr.contiguous()
+        kv_indptr = kv_indptr if kv_indptr.is_contiguous() else kv_indptr.contiguous()
+        batched = (kv_indptr.data_ptr(), batch_indices.data_ptr(), code, kv_indptr.shape[0] - 1)
     if cache.page_size == 0 and num_tokens:
         raise ValueError("the cache's pages have no slots")
     keep = (positions, kv_indices, kv_indptr, batch_indices)
-    args = (kv_indices.data_ptr(), _lib.dtype_code(kv_indices), kv_indices.shape[0], _lib.ptr(kv_indptr),
-            _lib.ptr(batch_indices), _lib.dtype_code(batch_indices) if batch_indices is not None else 0,
-            kv_indptr.shape[0] - 1 if kv_indptr is not None else 0, positions.data_ptr(), _lib.dtype_code(positions))
-    return keep, args
+    return keep, (kv_indices.data_ptr(), idx_code, kv_indices.shape[0], *batched, positions.data_ptr(), pos_code)
 
 
 def append_paged_kv_fp4(
@@ -120,25 +111,30 @@ def append_paged_kv_fp4(
     of, and other out-of-range indices raise IndexError, at the next
     ``braidinfer_amd.check_device_status()``.  Tokens must have distinct slots."""
     tokens, heads, dim = k.shape[0], cache.num_kv_heads, cache.head_dim
-    for name, t in (("k", k), ("v", v)):
-        if tuple(t.shape) != (tokens, heads, dim):
-            raise ValueError(f"{name} of shape {tuple(t.shape)} does not match the cache's [tokens, {heads}, {dim}] rows")
+    shape = (tokens, heads, dim)
+    if k.shape != shape or v.shape != shape:
+        name, t = ("k", k) if k.shape != shape else ("v", v)
+        raise ValueError(f"{name} of shape {tuple(t.shape)} does not match the cache's [tokens, {heads}, {dim}] rows")
     if k.dtype != v.dtype:
         raise TypeError(f"k and v must share a dtype (got {k.dtype} and {v.dtype})")
-    code = _lib.dtype_code(k)
-    if code > _lib.BF16:
+    code = _FLOATS.get(k.dtype)
+    if code is None:
         raise TypeError(f"k and v must be bf16, fp16 or fp32, not {k.dtype}")
-    k = k if k.stride(2) == 1 else k.contiguous()
-    v = v if v.stride(2) == 1 else v.contiguous()
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
+        k, v = k.contiguous(), v.contiguous()
+        ks, vs = k.stride(), v.stride()
     keep, where = _tokens(cache, kv_indices, kv_indptr, batch_indices, positions, tokens)
     dev = _lib.require_device(k, v, cache.codes, cache.scales, *keep)
     if tokens == 0:
         return
     with _lib.on_device(dev):
-        _lib.call("bfa_append_paged_kv_fp4", k.data_ptr(), v.data_ptr(), code, tokens, heads, dim,
-                  k.stride(0), k.stride(1), v.stride(0), v.stride(1), cache.codes.data_ptr(), cache.scales.data_ptr(),
-                  cache.num_pages, cache.page_size, *cache.codes.stride()[:4], *cache.scales.stride()[:4], *where,
-                  _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+        rc = _lib.entry("bfa_append_paged_kv_fp4")(
+            k.data_ptr(), v.data_ptr(), code, tokens, heads, dim, ks[0], ks[1], vs[0], vs[1], cache.codes.data_ptr(),
+            cache.scales.data_ptr(), cache.num_pages, cache.page_size, *cache.strides, *where,
+            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+    if rc < 0:
+        _lib.raise_error(rc)
 
 
 def gather_paged_kv_fp4(
@@ -154,17 +150,19 @@ def gather_paged_kv_fp4(
     16-bit cache, or to compare with what was stored).  bf16 and fp32 hold every value
     exactly, but for 2^128, to which magnitudes from 3.5 x 2^126 round: it reads as
     infinity, and in fp16 so does all that is past its range.  A token without a place, and padding, reads as zeros."""
-    code = _lib.dtype_code(dtype)
-    if code > _lib.BF16:
+    code = _FLOATS.get(dtype)
+    if code is None:
         raise TypeError(f"dtype must be bf16, fp16 or fp32, not {dtype}")
     tokens, heads, dim = positions.shape[0], cache.num_kv_heads, cache.head_dim
     keep, where = _tokens(cache, kv_indices, kv_indptr, batch_indices, positions, tokens)
     dev = _lib.require_device(cache.codes, cache.scales, *keep)
-    k, v = (torch.empty(tokens, heads, dim, dtype=dtype, device=dev) for _ in range(2))
+    k, v = torch.empty((2, tokens, heads, dim), dtype=dtype, device=dev).unbind()
     if tokens == 0:
         return k, v
     with _lib.on_device(dev):
-        _lib.call("bfa_gather_paged_kv_fp4", cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages,
-                  cache.page_size, heads, dim, *cache.codes.stride()[:4], *cache.scales.stride()[:4], *where, tokens,
-                  k.data_ptr(), v.data_ptr(), code, _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+        rc = _lib.entry("bfa_gather_paged_kv_fp4")(
+            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, cache.page_size, heads, dim, *cache.strides,
+            *where, tokens, k.data_ptr(), v.data_ptr(), code, _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+    if rc < 0:
+        _lib.raise_error(rc)
     return k, v

@@ -29,7 +29,7 @@ class PagedKVBatch(NamedTuple):
 
 
 _DTYPES = (torch.int32, torch.int32, torch.int32, torch.int32, torch.int32, torch.int64, torch.int64)
-_INTS = (torch.int32, torch.int64)
+_INTS = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 
 def build_paged_kv_batch(
@@ -53,12 +53,14 @@ def build_paged_kv_batch(
     if page_tables.dim() != 2:
         raise ValueError("page_tables must be [requests, max_pages]")
     seqs, width = page_tables.shape
-    for name, t in (("seq_lens", seq_lens), ("query_lens", query_lens)):
-        if t.dim() != 1 or t.shape[0] != seqs:
+    codes = []
+    for name, t, dims in (("seq_lens", seq_lens, 1), ("query_lens", query_lens, 1), ("page_tables", page_tables, 2)):
+        if t.dim() != dims or t.shape[0] != seqs:
             raise ValueError(f"{name} of shape {tuple(t.shape)} for {seqs} requests")
-    for name, t in (("page_tables", page_tables), ("seq_lens", seq_lens), ("query_lens", query_lens)):
-        if t.dtype not in _INTS:
+        code = _INTS.get(t.dtype)
+        if code is None:
             raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
+        codes.append(code)
     if page_size <= 0:
         raise ValueError("page_size must be positive")
     if num_tokens < 0:
@@ -69,16 +71,19 @@ def build_paged_kv_batch(
     dev = _lib.require_device(page_tables, seq_lens, query_lens)
     sizes = (seqs + 1, seqs + 1, seqs * width, seqs, num_tokens, num_tokens, num_tokens)
     if out is None:
-        out = PagedKVBatch(*(torch.empty(n, dtype=d, device=dev) for n, d in zip(sizes, _DTYPES)))
+        # two allocations for the seven (one of 1.4 us each otherwise)
+        out = PagedKVBatch(*torch.empty(sum(sizes[:5]), dtype=torch.int32, device=dev).split_with_sizes(sizes[:5]),
+                           *torch.empty(2, num_tokens, dtype=torch.int64, device=dev).unbind())
     else:
         for name, t, n, d in zip(out._fields, out, sizes, _DTYPES):
             if t.dtype != d or tuple(t.shape) != (n,) or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be a contiguous {d} tensor of {n} elements")
         _lib.require_device(page_tables, *out)
     with _lib.on_device(dev):
-        _lib.call("bfa_build_paged_kv_batch",
-                  page_tables.data_ptr(), _lib.dtype_code(page_tables), seqs, width, page_tables.stride(0),
-                  seq_lens.data_ptr(), _lib.dtype_code(seq_lens), query_lens.data_ptr(), _lib.dtype_code(query_lens),
-                  int(page_size), num_tokens, seqs * width, *(t.data_ptr() for t in out),
-                  _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+        rc = _lib.entry("bfa_build_paged_kv_batch")(
+            page_tables.data_ptr(), codes[2], seqs, width, page_tables.stride(0), seq_lens.data_ptr(), codes[0],
+            query_lens.data_ptr(), codes[1], int(page_size), num_tokens, seqs * width, *[t.data_ptr() for t in out],
+            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+    if rc < 0:
+        _lib.raise_error(rc)
     return out

@@ -17,16 +17,22 @@ from ..kernels.fp4_kv_cache import Fp4KVCache
 _LAYOUT_DIMS = {"HND": (2, 3), "NHD": (3, 2)}  # (head dim, slot dim) of the 5-D layer cache
 
 
-def _aligned(t: torch.Tensor, unit: int) -> bool:
-    """16-byte aligned, with strides (but the last, which is 1) in multiples of `unit`."""
-    st = t.stride()
-    return st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s, n in zip(st[:-1], t.shape) if n > 1)
+_QUERY = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _strides(t: torch.Tensor, dims) -> list[int]:
-    """Strides along `dims`, 0 for a dimension of one element (whose stride means nothing)."""
+def _strides(t: torch.Tensor, unit: int):
+    """Strides of t, multiples of `unit` but for the last, which is 1, and 16-byte
+    aligned; None if they are not.  0 for a dimension of one element, whose stride means
+    nothing, where it is not such a multiple."""
     st = t.stride()
-    return [st[i] if t.shape[i] > 1 else 0 for i in dims]
+    bits = 0
+    for s in st[:-1]:
+        bits |= s
+    if bits % unit:
+        st = tuple(0 if n == 1 else s for n, s in zip(t.shape[:-1], st)) + st[-1:]
+        if any(s % unit for s in st[:-1]):
+            return None
+    return st if st[-1] == 1 and t.data_ptr() % 16 == 0 else None
 
 
 def paged_attention(
@@ -62,28 +68,30 @@ def paged_attention(
     if query.dim() != 3:
         raise ValueError(f"query of shape {tuple(query.shape)} is not [tokens, heads, head_dim]")
     tokens, hq, dim = query.shape
-    code = _lib.dtype_code(query)
-    if code not in (_lib.BF16, _lib.F16):
-        raise TypeError(f"query must be bf16 or fp16, not {query.dtype}")
-    if isinstance(kv_cache, Fp4KVCache):
-        data, scales, cache_code = kv_cache.codes, kv_cache.scales, _lib.FP4
+    dtype = query.dtype
+    code = _QUERY.get(dtype)
+    if code is None:
+        raise TypeError(f"query must be bf16 or fp16, not {dtype}")
+    if type(kv_cache) is Fp4KVCache:
         if kv_layout != "HND":
             raise ValueError("a 4-bit cache has layout HND")
+        data, scales, cache_code, unit = kv_cache.codes, kv_cache.scales, _lib.FP4, 16
         pages, hkv, slots, cache_dim = kv_cache.num_pages, kv_cache.num_kv_heads, kv_cache.page_size, kv_cache.head_dim
-        st, sst = _strides(data, (0, 1, 2, 3)), _strides(scales, (0, 1, 2, 3))
-        unit = 16
+        h, s = 2, 3
+        sst = kv_cache.strides[4:]
     else:
-        if kv_layout not in _LAYOUT_DIMS:
+        dims = _LAYOUT_DIMS.get(kv_layout)
+        if dims is None:
             raise ValueError(f"Unknown kv_layout: {kv_layout}")
-        if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
+        h, s = dims
+        data, scales, cache_code, unit = kv_cache, None, code, 8
+        shape = data.shape
+        if len(shape) != 5 or shape[1] != 2:
             raise ValueError("kv_cache must be one layer [num_pages, 2, ...] with 5 dimensions")
-        if kv_cache.dtype != query.dtype:
-            raise TypeError(f"query and kv_cache must share a dtype (got {query.dtype} and {kv_cache.dtype})")
-        h, s = _LAYOUT_DIMS[kv_layout]
-        data, scales, cache_code = kv_cache, None, code
-        pages, hkv, slots, cache_dim = kv_cache.shape[0], kv_cache.shape[h], kv_cache.shape[s], kv_cache.shape[4]
-        st, sst = _strides(data, (0, 1, h, s)), (0, 0, 0, 0)
-        unit = 8
+        if data.dtype != dtype:
+            raise TypeError(f"query and kv_cache must share a dtype (got {dtype} and {data.dtype})")
+        pages, hkv, slots, cache_dim = shape[0], shape[h], shape[s], shape[4]
+        sst = (0, 0, 0, 0)
     if cache_dim != dim:
         raise ValueError(f"kv_cache holds rows of {cache_dim} elements, query of {dim}")
     if dim not in (64, 128):
@@ -92,45 +100,55 @@ def paged_attention(
         raise ValueError(f"{hq} query heads do not share {hkv} kv heads evenly")
     if slots == 0:
         raise ValueError("the cache's pages have no slots")
-    if pages and not _aligned(data, unit):
-        raise ValueError("kv_cache must be 16-byte aligned, with unit stride along head_dim and others in multiples of 16 bytes")
-    if window is not None and window < 1:
+    st = _strides(data, unit)
+    if st is None:
+        if pages:
+            raise ValueError("kv_cache must be 16-byte aligned, with unit stride along head_dim and others in multiples of "
+                             "16 bytes")
+        st = (0, 0, 0, 0)
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError("window must be at least 1 (None for no window)")
     if num_sinks < 0:
         raise ValueError("num_sinks must not be negative")
-    seqs = kv_last_page_len.shape[0] if kv_last_page_len.dim() == 1 else -1
-    lists = []
-    for name, t, n in (("kv_indices", kv_indices, None), ("kv_indptr", kv_indptr, seqs + 1),
-                       ("kv_last_page_len", kv_last_page_len, seqs), ("qo_indptr", qo_indptr, seqs + 1)):
-        if t.dtype != torch.int32 or t.dim() != 1:
-            raise TypeError(f"{name} must be a one-dimensional int32 tensor")
-        if n is not None and t.shape[0] != n:
-            raise ValueError(f"{name} has {t.shape[0]} elements, for {seqs} requests {n} are needed")
-        lists.append(t if t.is_contiguous() else t.contiguous())
-    kv_indices, kv_indptr, kv_last_page_len, qo_indptr = lists
-    if not _aligned(query, 8):
-        query = query.contiguous()
-        if query.data_ptr() % 16:
-            query = query.clone()
-    dev = _lib.require_device(query, data, scales, *lists, out)
+    if (kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_last_page_len.dtype != torch.int32
+            or qo_indptr.dtype != torch.int32 or kv_indices.dim() != 1 or kv_indptr.dim() != 1
+            or kv_last_page_len.dim() != 1 or qo_indptr.dim() != 1):
+        raise TypeError("kv_indices, kv_indptr, kv_last_page_len and qo_indptr must be one-dimensional int32 tensors")
+    seqs, num_indices = kv_last_page_len.shape[0], kv_indices.shape[0]
+    if kv_indptr.shape[0] != seqs + 1 or qo_indptr.shape[0] != seqs + 1:
+        name, t = ("kv_indptr", kv_indptr) if kv_indptr.shape[0] != seqs + 1 else ("qo_indptr", qo_indptr)
+        raise ValueError(f"{name} has {t.shape[0]} elements, for {seqs} requests {seqs + 1} are needed")
+    kv_indices, kv_indptr = kv_indices.contiguous(), kv_indptr.contiguous()
+    kv_last_page_len, qo_indptr = kv_last_page_len.contiguous(), qo_indptr.contiguous()
+    qs = _strides(query, 8)
+    if qs is None:
+        query = query.clone(memory_format=torch.contiguous_format)
+        qs = query.stride()
+    dev = _lib.require_device(query, data, scales, kv_indices, kv_indptr, kv_last_page_len, qo_indptr, out)
+    row = hq * dim
     if out is None:
-        out = torch.empty(tokens, hq * dim, dtype=query.dtype, device=dev)
-    elif out.dtype != query.dtype or tuple(out.shape) != (tokens, hq * dim) or not _aligned(out, 8):
-        raise ValueError(f"out must be a 16-byte aligned [{tokens}, {hq * dim}] tensor of the query's dtype, its row "
-                         "stride a multiple of 8")
+        out = torch.empty((tokens, row), dtype=dtype, device=dev)
+    else:
+        ost = _strides(out, 8) if out.dtype == dtype and tuple(out.shape) == (tokens, row) else None
+        if ost is None:
+            raise ValueError(f"out must be a 16-byte aligned [{tokens}, {row}] tensor of the query's dtype, its row stride a "
+                             "multiple of 8")
+        row = ost[0]
     if tokens == 0 or seqs == 0:
         return out
-    win = 0 if window is None else int(window)
-    size = _lib.workspace_size("bfa_paged_attention_workspace_size", tokens, seqs, hq, hkv, dim, kv_indices.shape[0], slots,
-                               win, int(num_sinks), cache_code)
-    qs = _strides(query, (0, 1))
+    size = _lib.entry("bfa_paged_attention_workspace_size")(tokens, seqs, hq, hkv, dim, num_indices, slots, window, num_sinks,
+                                                            cache_code)
     ws = _lib.scratch(dev)
     with _lib.on_device(dev), ws.lock:
         ws.reserve(size)
-        _lib.call("bfa_paged_attention", query.data_ptr(), code, tokens, hq, qs[0], qs[1], data.data_ptr(), cache_code,
-                  pages, hkv, slots, dim, *st, _lib.ptr(scales), *sst, kv_indices.data_ptr(), kv_indices.shape[0],
-                  kv_indptr.data_ptr(), kv_last_page_len.data_ptr(), qo_indptr.data_ptr(), seqs,
-                  dim ** -0.5 if scale is None else float(scale), win, int(num_sinks), out.data_ptr(),
-                  out.stride(0) if tokens > 1 else hq * dim, ws.ptr, ws.size, _lib.status_word(dev).data_ptr(),
-                  _lib.stream_of(dev))
+        rc = _lib.entry("bfa_paged_attention")(
+            query.data_ptr(), code, tokens, hq, qs[0], qs[1], data.data_ptr(), cache_code, pages, hkv, slots, dim, st[0],
+            st[1], st[h], st[s], None if scales is None else scales.data_ptr(), *sst, kv_indices.data_ptr(), num_indices,
+            kv_indptr.data_ptr(), kv_last_page_len.data_ptr(), qo_indptr.data_ptr(), seqs,
+            dim ** -0.5 if scale is None else float(scale), window, num_sinks, out.data_ptr(), row, ws.ptr, ws.size,
+            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+    if rc < 0:
+        _lib.raise_error(rc)
     return out

@@ -34,44 +34,67 @@ def qk_norm_rope(
     if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype != torch.float32:
         raise ValueError("cos_sin_cache must be float32 [max_position, head_dim]")
     max_position, dim = cos_sin_cache.shape
-    tokens = positions.shape[0] if positions.dim() == 1 else -1
-    if tokens < 0 or positions.dtype not in (torch.int32, torch.int64):
+    pos_code = _INTS.get(positions.dtype)
+    if pos_code is None or positions.dim() != 1:
         raise ValueError("positions must be a one-dimensional int32 or int64 tensor")
+    tokens = positions.shape[0]
     if dim == 0 or dim % 2:
         raise ValueError(f"head_dim {dim} must be even")
-    rows = []
-    for name, x in (("query", query), ("key", key)):
-        if x.dim() == 2 and x.shape[0] == tokens and x.shape[1] % dim == 0:
-            rows.append((x if x.stride(1) == 1 else x.contiguous()).unflatten(1, (-1, dim)))
-        elif x.dim() == 3 and x.shape[0] == tokens and x.shape[2] == dim:
-            rows.append(x if x.stride(2) == 1 else x.contiguous())
-        else:
-            raise ValueError(f"{name} of shape {tuple(x.shape)} is not [{tokens}, heads * {dim}] or [{tokens}, heads, {dim}]")
-    q, k = rows
-    if q.dtype != k.dtype:
-        raise TypeError(f"query and key must share a dtype (got {q.dtype} and {k.dtype})")
-    code = _lib.dtype_code(q)
-    if code > _lib.BF16:
-        raise TypeError(f"query and key must be bf16, fp16 or fp32, not {q.dtype}")
-    weights = [w.detach().contiguous() if w is not None else None for w in (q_norm_weight, k_norm_weight)]
-    given = [w for w in weights if w is not None]
-    w_code = _lib.F32
-    if given:
-        if any(w.numel() != dim for w in given):
+    if query.dtype != key.dtype:
+        raise TypeError(f"query and key must share a dtype (got {query.dtype} and {key.dtype})")
+    code = _FLOATS.get(query.dtype)
+    if code is None:
+        raise TypeError(f"query and key must be bf16, fp16 or fp32, not {query.dtype}")
+    q, q_heads, q_token, q_head = _rows("query", query, tokens, dim)
+    k, k_heads, k_token, k_head = _rows("key", key, tokens, dim)
+    w_code = None
+    ptrs = []
+    for w in (q_norm_weight, k_norm_weight):
+        if w is None:
+            ptrs.append((None, None))
+            continue
+        if w.numel() != dim:
             raise ValueError(f"norm weights must have head_dim = {dim} elements")
-        w_code = _lib.dtype_code(given[0])
-        if given[0].dtype != given[-1].dtype or w_code > _lib.BF16:
+        c = _FLOATS.get(w.dtype)
+        if c is None or w_code not in (None, c):
             raise TypeError("norm weights must share a dtype: bf16, fp16 or fp32")
-    positions, cos_sin_cache = positions.contiguous(), cos_sin_cache.contiguous()
-    dev = _lib.require_device(q, k, positions, cos_sin_cache, *given)
+        w_code = c
+        if not w.is_contiguous():
+            w = w.detach().contiguous()
+        ptrs.append((w, w.data_ptr()))
+    (qw, qw_ptr), (kw, kw_ptr) = ptrs
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if not cos_sin_cache.is_contiguous():
+        cos_sin_cache = cos_sin_cache.contiguous()
+    dev = _lib.require_device(q, k, positions, cos_sin_cache, qw, kw)
     q_out = torch.empty(query.shape, dtype=q.dtype, device=dev)
     k_out = torch.empty(key.shape, dtype=k.dtype, device=dev)
     if tokens == 0:
         return q_out, k_out
     with _lib.on_device(dev):
-        _lib.call("bfa_qk_norm_rope", q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), q_out.data_ptr(),
-                  k.data_ptr(), k.shape[1], k.stride(0), k.stride(1), k_out.data_ptr(), code, tokens, dim,
-                  _lib.ptr(weights[0]), _lib.ptr(weights[1]), w_code, float(eps), positions.data_ptr(),
-                  _lib.dtype_code(positions), cos_sin_cache.data_ptr(), max_position,
-                  _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+        rc = _lib.entry("bfa_qk_norm_rope")(
+            q.data_ptr(), q_heads, q_token, q_head, q_out.data_ptr(), k.data_ptr(), k_heads, k_token, k_head,
+            k_out.data_ptr(), code, tokens, dim, qw_ptr, kw_ptr, w_code or 0, float(eps), positions.data_ptr(), pos_code,
+            cos_sin_cache.data_ptr(), max_position, _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
+    if rc < 0:
+        _lib.raise_error(rc)
     return q_out, k_out
+
+
+_INTS = {torch.int32: _lib.I32, torch.int64: _lib.I64}
+_FLOATS = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _rows(name: str, x: torch.Tensor, tokens: int, dim: int):
+    """(x with unit stride along a head's row, heads, token stride, head stride)"""
+    shape = x.shape
+    if len(shape) == 2 and shape[0] == tokens and shape[1] % dim == 0:
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        return x, shape[1] // dim, x.stride(0), dim
+    if len(shape) == 3 and shape[0] == tokens and shape[2] == dim:
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        return x, shape[1], x.stride(0), x.stride(1)
+    raise ValueError(f"{name} of shape {tuple(shape)} is not [{tokens}, heads * {dim}] or [{tokens}, heads, {dim}]")

@@ -86,7 +86,10 @@ const char* bfa_last_error(void);
 #define BFA_TUNE_GEMM_SPLITS 14      /* BFA_GEMM_SPLITS: K splits of their tiles past whole rounds */
 #define BFA_TUNE_LINEAR_GEMV 15      /* BFA_LINEAR_GEMV: 0 = never the one-launch linear kernel,
                                         non-zero = for every call of up to 64 tokens */
-#define BFA_TUNE_COUNT 16
+#define BFA_TUNE_PAGED_ROWS 16       /* BFA_PAGED_ROWS: rows of a block of the paged attention:
+                                        16 (the decode form), 64 or 128 */
+#define BFA_TUNE_PAGED_WG 17         /* BFA_PAGED_WG: workgroup target of its key split, 0 = unsplit */
+#define BFA_TUNE_COUNT 18
 int bfa_set_tuning(int key, int value);
 int bfa_get_tuning(int key);
 

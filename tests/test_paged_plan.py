@@ -34,6 +34,7 @@ int split(int qlen, int kvlen, int group, int bm, int window, int sinks, int til
   return p.tiles;
 }
 int chunks(int blocks, int tiles, int per) { return PagedSplit{blocks, tiles}.chunks(per); }
+int even(int tiles, int chunks) { return paged_even(tiles, chunks); }
 int per_item(long long total, int target, int least) { return paged_per_item(total, target, least); }
 }
 """
@@ -145,5 +146,9 @@ def test_items_cover_every_block(lib):
         assert all(lib.chunks(b, t, per) * per >= t for b, t in plans)
         rows = sum(q for q, _ in requests) * group
         assert sum(b for b, _ in plans) <= min(rows, rows // bm + len(requests))
+        for _, t in plans:
+            c = lib.chunks(1, t, per)
+            assert t <= lib.even(t, c) * c and (c == 1 or lib.even(t, c) <= per)
+    assert lib.even(0, 1) == 0 and lib.even(2 ** 31 - 1, 1) == 2 ** 31 - 1 and lib.even(7, 3) == 3
     assert lib.chunks(1, 0, 4) == 1 and lib.chunks(1, 2 ** 31 - 1, 2 ** 31 - 1) == 1
     assert lib.per_item(2 ** 60, 1, 2) == 0x3fffffff
