@@ -187,7 +187,7 @@ __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float sl2, floa
                                        pa_f32x4_t (&o)[RB][D / 16], const uint4* vt, int lane) {
   constexpr int OJ = D / 16;
   constexpr float LAG = 6.f;
-  uint4 pf[RB][KC / 2];
+  float mul[RB], ref[RB], sum[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     float mx = -INFINITY;
@@ -204,39 +204,53 @@ __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float sl2, floa
 #pragma unroll
       for (int j = 0; j < OJ; ++j) o[rb][j] *= alpha;
     }
-    const float ref = m[rb] == -INFINITY ? 0.f : m[rb];
-    float sum = 0.f;
-    if (__any(fabsf(ref) >= 65536.f)) {
+    ref[rb] = m[rb] == -INFINITY ? 0.f : m[rb];
+    mul[rb] = sl2;
+    sum[rb] = 0.f;
+    if (__any(fabsf(ref[rb]) >= 65536.f)) {
 #pragma unroll
       for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[rb][c][i] = __builtin_amdgcn_exp2f(sc[rb][c][i] * sl2 - ref);
-    } else {
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[rb][c][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][c][i], sl2, -ref));
+        for (int i = 0; i < 4; ++i) sc[rb][c][i] = sc[rb][c][i] * sl2 - ref[rb];
+      mul[rb] = 1.f, ref[rb] = 0.f;
     }
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += sc[rb][c][i];
-    l[rb] += sum;
-#pragma unroll
-    for (int h = 0; h < KC / 2; ++h)
-      pf[rb][h] = make_uint4(pa_pack<BF16>(sc[rb][2 * h][0], sc[rb][2 * h][1]),
-                             pa_pack<BF16>(sc[rb][2 * h][2], sc[rb][2 * h][3]),
-                             pa_pack<BF16>(sc[rb][2 * h + 1][0], sc[rb][2 * h + 1][1]),
-                             pa_pack<BF16>(sc[rb][2 * h + 1][2], sc[rb][2 * h + 1][3]));
   }
+  // The weights of the first 32 keys, then their products with V between the weights of
+  // the next 32: the matrix core works while the wave computes exponentials.
+  auto weight = [&](int rb, int c, int i) {
+    sc[rb][c][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][c][i], mul[rb], -ref[rb]));
+    sum[rb] += sc[rb][c][i];
+  };
+  uint4 pf[RB];
 #pragma unroll
-  for (int h = 0; h < KC / 2; ++h)
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) weight(rb, c, i);
+#pragma unroll
+  for (int h = 0; h < KC / 2; ++h) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      pf[rb] = make_uint4(pa_pack<BF16>(sc[rb][2 * h][0], sc[rb][2 * h][1]),
+                          pa_pack<BF16>(sc[rb][2 * h][2], sc[rb][2 * h][3]),
+                          pa_pack<BF16>(sc[rb][2 * h + 1][0], sc[rb][2 * h + 1][1]),
+                          pa_pack<BF16>(sc[rb][2 * h + 1][2], sc[rb][2 * h + 1][3]));
 #pragma unroll
     for (int j = 0; j < OJ; ++j) {
       const uint4 vf = v_fragment<D>(vt, 32 * h, j, lane);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) o[rb][j] = pa_mfma<BF16>(vf, pf[rb][h], o[rb][j]);
+      for (int rb = 0; rb < RB; ++rb) o[rb][j] = pa_mfma<BF16>(vf, pf[rb], o[rb][j]);
+      if (h + 1 < KC / 2) {  // 8 weights of each row block over the OJ steps
+#pragma unroll
+        for (int w = 8 / OJ * j; w < 8 / OJ * (j + 1); ++w)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) weight(rb, 2 * h + 2 + w / 4, w % 4);
+      }
     }
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) l[rb] += sum[rb];
 }
 
 // Scores of keys that a row does not see, or that do not exist, to -inf whatever they
@@ -782,11 +796,29 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   const uint8_t* ksc = FP4 ? a.scales + h * a.s_sh : nullptr;
   const uint32_t cstride = a.c_ss * 16;
   using Keys = KeyTile<FP4, P16, KT>;
+  // 16-bit rows of P16 pages go to the LDS by DMA, 64 granules in the order of their
+  // slots an instruction (a lane fetches the granule that belongs in its slot: f(r) of
+  // its row is the same in every load); the others through registers.
+  constexpr bool DMA = !FP4 && P16;
+  const uint32_t kl = lds_addr(kbuf), vl = lds_addr(vbuf);
+  const uint32_t koff = DMA ? sub * cstride + 16 * k_slot<D>(row0_of(0) + sub, part) : 0;
+  const uint32_t voff = DMA ? sub * cstride + 16 * v_slot<D>(row0_of(0) + sub, part) : 0;
   struct Tile {
     Code k[NL], v[NL];
     uint32_t ks, vs;
   };
   auto entry = [&](int32_t i) { return Keys::entry(a, it.s, kt.at(min(i, kt.count - 1)) * KT, lane); };
+  auto copy = [&](const Keys& keys, int b) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int r0 = row0_of(n);
+      const uint8_t* p = kbase + static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(keys.kr.off), r0 / 16))) * 16 +
+                         static_cast<uint32_t>(r0 % 16) * cstride;
+      const uint32_t at = (b * KT + r0) * GK * 16;
+      dma16(p, koff, kl + at);
+      dma16(p + a.c_skv, voff, vl + at);
+    }
+  };
   auto issue = [&](const Keys& keys) {
     Tile t;
 #pragma unroll
@@ -833,6 +865,28 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
       }
     }
   };
+  // the same for a tile that is in the LDS already
+  auto mend = [&](int b, uint64_t exists, bool edge) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int r = row0_of(n) + sub, at = r * GK + part;
+      const bool ok = (exists >> r) & 1;
+      uint4 v = vbuf[b][at];
+      if (!ok) kbuf[b][at] = vbuf[b][at] = make_uint4(0, 0, 0, 0);
+      else if (edge && pa_make_finite<BF16>(v)) odd = true, vbuf[b][at] = v;
+    }
+    __syncthreads();
+  };
+  // a tile has arrived in buffer b, and every wave is done with the other
+  auto arrive = [&](int b, uint64_t exists, bool edge) {
+    if constexpr (DMA) {
+      wait_vmem();
+      __syncthreads();
+      if (edge || exists != Keys::all()) mend(b, exists, edge);
+    } else {
+      __syncthreads();
+    }
+  };
   auto wg_edge = [&](int32_t i) {
     return tile_edge(kt.at(i) * KT, KT, rows.first, rows.last, a.window, a.sinks);
   };
@@ -841,20 +895,22 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
     Tile cur;
     {
       const Keys keys(a, it.s, kt.at(i0) * KT, entry(i0), lane);
-      cur = issue(keys);
       exists = ahead = keys.exists;
+      if constexpr (DMA) copy(keys, 0);
+      else cur = issue(keys);
     }
     int32_t id = entry(i0 + 1);
-    store(cur, 0, exists, wg_edge(i0));
-    __syncthreads();
+    if constexpr (!DMA) store(cur, 0, exists, wg_edge(i0));
+    arrive(0, exists, wg_edge(i0));
     for (int32_t i = i0; i < i1; ++i) {
       const int b = (i - i0) & 1;
       const bool more = i + 1 < i1;
       const int32_t id2 = entry(i + 2);
       if (more) {
         const Keys keys(a, it.s, kt.at(i + 1) * KT, id, lane);
-        cur = issue(keys);
         ahead = keys.exists;
+        if constexpr (DMA) copy(keys, b ^ 1);
+        else cur = issue(keys);
       }
       id = id2;
       const int32_t key0 = kt.at(i) * KT;
@@ -879,9 +935,9 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
         attend<BF16, D, KC, RB>(sc, a.sl2, m, l, o, vbuf[b], lane);
       }
       if (more) {
-        store(cur, b ^ 1, ahead, wg_edge(i + 1));
+        if constexpr (!DMA) store(cur, b ^ 1, ahead, wg_edge(i + 1));
         exists = ahead;
-        __syncthreads();  // the tile is whole, and every wave is done with the other
+        arrive(b ^ 1, exists, wg_edge(i + 1));
       }
     }
     if (__syncthreads_or(odd)) poison<BF16, D, FP4, KT, RB>(a, it.s, rows.first, rows.last, kt, i0, i1, 1, h, hi, lo, o, lane);
