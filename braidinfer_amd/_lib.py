@@ -362,25 +362,24 @@ def stream_of(device: torch.device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class _Here:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """A context in which launches go to `device`: its default stream's handle is null,
-    which a launch takes for the current device's.  torch.cuda.device() where it is
-    another one, and nothing (it takes 3 us) where it is current."""
+def launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, status word, stream) of an entry point with `device` current: its default
+    stream's handle is null, which a launch takes for the current device's.  Raises on a
+    negative return."""
     idx = device.index
-    return _HERE if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(device)
+    word = _status.get(idx)
+    if word is None:
+        word = status_word(device)
+    if idx is None or idx == _raw_device():
+        rc = fn(*args, word.data_ptr(), stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, word.data_ptr(), stream_of(device))
+    if rc < 0:
+        raise_error(rc)
 
 
 _status: dict[int, torch.Tensor] = {}

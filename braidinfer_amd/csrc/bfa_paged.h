@@ -52,60 +52,93 @@ BFA_HD int64_t paged_page(int64_t id, int64_t num_pages) {
   return id >= 0 && id < num_pages ? id : -1;
 }
 
-// The key tiles (of `tile` keys) that any row at positions first .. last sees, in
-// order: `sinks` tiles from the front, then those from tile `from` on; count in all.
+// What the cut depends on beside the lengths: `bm` rows to a block (a row is a query
+// token and one of the `group` heads of a kv head), `tile` keys to a tile (a power of
+// two), the window (0 for none) and the sinks, in whole tiles.
+struct PagedShape {
+  int32_t bm, group, tile;
+  int32_t window, sink_tiles;
+  int32_t most;  // bound of a block's key tiles from its window
+};
+
+BFA_HD PagedShape paged_shape(int32_t bm, int32_t group, int32_t tile, int32_t window, int32_t sinks) {
+  PagedShape p{bm, group, tile, window, 0, 0x7fffffff};
+  p.sink_tiles = sinks / tile + (sinks % tile != 0);
+  if (window > 0) {
+    // one block's rows lie within (bm - 1) / group + 2 tokens: its window's keys within
+    // that many more, on two tiles more than they fill, and the sinks' tiles
+    const int64_t keys = static_cast<int64_t>(window) + bm / group + 2;
+    const int64_t most = keys / tile + 2 + p.sink_tiles;
+    if (most < p.most) p.most = static_cast<int32_t>(most);
+  }
+  return p;
+}
+
+// The key tiles that any row at positions first .. last sees, in order: `sinks` tiles
+// from the front, then those from tile `from` on; count in all.
 struct KeyTiles {
   int32_t sinks, from, count;
   BFA_HD int32_t at(int32_t i) const { return i < sinks ? i : from + (i - sinks); }
 };
 
-// window: 0 for none.  first and last may be negative (rows before the cache's
-// first token, which see nothing).
-BFA_HD KeyTiles paged_key_tiles(int32_t first, int32_t last, int32_t kvlen, int32_t window, int32_t sinks,
-                                int32_t tile) {
+// first and last may be negative (rows before the cache's first token, which see
+// nothing).
+BFA_HD KeyTiles paged_key_tiles(int32_t first, int32_t last, int32_t kvlen, const PagedShape& p) {
   KeyTiles k{0, 0, 0};
   if (last >= kvlen) last = kvlen - 1;
   if (last < 0) return k;
-  const int32_t all = last / tile + 1;
-  if (window > 0 && first >= window) {
-    k.from = (first - window + 1) / tile;
-    const int32_t s = sinks / tile + (sinks % tile != 0);
-    k.sinks = s < k.from ? s : k.from;
+  const uint32_t tile = static_cast<uint32_t>(p.tile);
+  const int32_t all = static_cast<int32_t>(static_cast<uint32_t>(last) / tile) + 1;
+  if (p.window > 0 && first >= p.window) {
+    k.from = static_cast<int32_t>(static_cast<uint32_t>(first - p.window + 1) / tile);
+    k.sinks = p.sink_tiles < k.from ? p.sink_tiles : k.from;
   }
   k.count = k.sinks + all - k.from;
   return k;
 }
 
-// Work items.  Request s has `blocks` blocks of `bm` rows (a row is a query token
-// and one of the `group` heads of a kv head), each over at most `tiles` key tiles;
-// with `per` key tiles to an item a block takes ceil(tiles / per) items.
+// Work items.  Request s has `blocks` blocks of rows, each over at most `tiles` key
+// tiles; with `per` key tiles to an item a block takes ceil(tiles / per) items.
 struct PagedSplit {
   int32_t blocks, tiles;
-  BFA_HD int32_t chunks(int32_t per) const { return tiles > 0 ? (tiles - 1) / per + 1 : 1; }
+  BFA_HD int32_t chunks(int32_t per) const {
+    return tiles > per ? static_cast<int32_t>((static_cast<uint32_t>(tiles) - 1) / static_cast<uint32_t>(per)) + 1 : 1;
+  }
 };
 
-BFA_HD PagedSplit paged_split(const PagedSeq& s, int32_t group, int32_t bm, int32_t window, int32_t sinks,
-                              int32_t tile) {
-  PagedSplit p{0, 0};
-  const int64_t rows = static_cast<int64_t>(s.qlen) * group;
-  p.blocks = static_cast<int32_t>((rows + bm - 1) / bm);
-  const int32_t first = s.kvlen - s.qlen;
-  p.tiles = paged_key_tiles(first, s.kvlen - 1, s.kvlen, window, sinks, tile).count;
-  if (window > 0) {
-    // one block's rows lie within ceil(bm / group) + 1 tokens: its window's keys
-    // within that many more, on one more tile than they fill, and the sinks' tiles
-    const int64_t keys = static_cast<int64_t>(window) + bm / group + 2;
-    const int64_t most = keys / tile + 2 + sinks / tile + 1;
-    if (most < p.tiles) p.tiles = static_cast<int32_t>(most);
-  }
-  return p;
+BFA_HD PagedSplit paged_split(const PagedSeq& s, const PagedShape& p) {
+  PagedSplit sp{0, 0};
+  const uint32_t rows = static_cast<uint32_t>(s.qlen) * static_cast<uint32_t>(p.group);  // < 2^30 (checked by the caller)
+  sp.blocks = static_cast<int32_t>((rows + p.bm - 1) / static_cast<uint32_t>(p.bm));
+  sp.tiles = paged_key_tiles(s.kvlen - s.qlen, s.kvlen - 1, s.kvlen, p).count;
+  if (sp.tiles > p.most) sp.tiles = p.most;
+  return sp;
 }
 
-// Key tiles to an item, so that `total` tiles (the sum of blocks * tiles) make at
-// most `target` items beside one for each block; at least `least`.
-BFA_HD int32_t paged_per_item(int64_t total, int32_t target, int32_t least) {
-  const int64_t per = (total + target - 1) / target;
-  return per < least ? least : static_cast<int32_t>(per > 0x3fffffff ? 0x3fffffff : per);
+// Work is summed in units of 2^shift key tiles, rounded up, so that the sum of all
+// requests stays below 2^30; sums are held there, which only broken offsets (whose
+// requests overlap) can reach.
+constexpr int32_t PAGED_MOST = 0x3fffffff;
+BFA_HD int32_t paged_work(const PagedSplit& s, int32_t shift) {
+  const int64_t w = static_cast<int64_t>(s.blocks) * (s.tiles > 0 ? ((s.tiles - 1) >> shift) + 1 : 0);
+  return w > PAGED_MOST ? PAGED_MOST : static_cast<int32_t>(w);
+}
+
+// Key tiles to an item, so that `work` units make at most `target` items beside one for
+// each block; at least `least`.
+BFA_HD int32_t paged_per_item(int32_t work, int32_t shift, int32_t target, int32_t least) {
+  const uint32_t units = (static_cast<uint32_t>(work) + target - 1) / static_cast<uint32_t>(target);
+  const int64_t per = static_cast<int64_t>(units) << shift;
+  return per < least ? least : static_cast<int32_t>(per > PAGED_MOST ? PAGED_MOST : per);
+}
+
+// Items of a request, held likewise.
+BFA_HD int32_t paged_items(const PagedSplit& s, int32_t per) {
+  const int64_t n = static_cast<int64_t>(s.blocks) * s.chunks(per);
+  return n > PAGED_MOST ? PAGED_MOST : static_cast<int32_t>(n);
+}
+BFA_HD int32_t paged_add(int32_t a, int32_t b) {  // of values up to PAGED_MOST
+  return a + b > PAGED_MOST ? PAGED_MOST : a + b;
 }
 
 // Key tiles of each of a block's `chunks` items, so that they are alike: with `per`

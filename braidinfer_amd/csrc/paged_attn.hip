@@ -65,11 +65,14 @@ struct PagedArgs {
   FastDiv group, ps, heads;       // Hq / Hkv, page size, Hkv
   float sl2, oscale;              // |scale| x log2(e) (1 for a scale of 0), factor of the output
   uint32_t qand, qxor;            // on pairs of query values: zero them, turn their signs
-  int32_t window, sinks;
+  PagedShape shape;
+  int32_t sinks;
   uint16_t* out;                  // [tokens, Hq * D], row stride out_st
   int64_t out_st;
-  int32_t split, target, least;   // 0: an item is a block
-  int32_t nblocks;                // bound of the blocks
+  int32_t split, target, least;   // split 0: an item is a block
+  int32_t shift;                  // of the sum of the work
+  int32_t nblocks, items;         // bounds of the blocks and the items
+  int4* plan;                     // [items, 2] the items, where a launch of its own finds them
   float* acc;                     // [items, Hkv, BM, D] partial sums
   float* ml;                      // [items, Hkv, BM, 2] their maxima and sums
   int4* table;                    // [nblocks] (first item, items, first query row, rows) of a block
@@ -290,101 +293,147 @@ __device__ __forceinline__ bool tile_edge(int32_t key0, int n, int32_t first, in
 // ------------------------------------------------------------------- items
 struct Item {
   PagedSeq s;
-  int32_t block, chunk, chunks, index;
-  bool live;
+  int32_t block, chunk, chunks;  // chunks 0: no item
 };
 
-// Inclusive sum over the lanes, held at SCAN_MOST: no request order, broken offsets
-// included, overflows it.  before(): what the lanes before hold.
-constexpr int32_t SCAN_MOST = 0x3fffffff;
-__device__ __forceinline__ int32_t scan_lanes(int32_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int32_t u = __shfl_up(v, d);
-    if (lane >= d) v = min(v + u, SCAN_MOST);
-  }
-  return v;
+// Inclusive sum over the lanes (row shifts, then the rows' last lanes broadcast), held
+// at PAGED_MOST; and what the lanes before hold.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t scan_step(int32_t v) {
+  return paged_add(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false));
 }
-__device__ __forceinline__ int32_t before(int32_t end, int lane) {
+__device__ __forceinline__ int32_t scan_lanes(int32_t v) {
+  v = scan_step<0x111, 0xF>(v);
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);
+  return scan_step<0x143, 0xC>(v);
+}
+__device__ __forceinline__ int32_t lane_before(int32_t end) {
   const int32_t u = __shfl_up(end, 1);
-  return lane == 0 ? 0 : u;
+  return (threadIdx.x & 63) == 0 ? 0 : u;
 }
 
-// Item x of the grid: every wave finds it by itself, 64 requests at a time, lane by
-// lane.  The first pass sums the work (the key tiles of all blocks), from which the
-// tiles to an item follow; the second finds the request that owns item x.  The
-// item's first workgroup fills the block's line of the table that the merge reads,
-// and workgroups past the last item the lines past the last block.
-template <int BM, int KT>
+__device__ __forceinline__ PagedSeq request(const PagedArgs& a, int32_t b, bool& bad) {
+  bad = false;
+  if (b >= a.num_seqs) return PagedSeq{0, 0, 0, 0, 0};
+  return paged_seq(a.qo_indptr[b], a.qo_indptr[b + 1], a.kv_indptr[b], a.kv_indptr[b + 1], a.last[b], a.tokens,
+                   a.num_indices, static_cast<int32_t>(a.ps.d), bad);
+}
+
+// the line of the table that the merge reads for a block
+__device__ __forceinline__ int4 table_line(const PagedArgs& a, const PagedSeq& s, int32_t block, int32_t chunks, int32_t item) {
+  const int32_t group = static_cast<int32_t>(a.group.d), row0 = block * a.shape.bm;
+  return make_int4(item, chunks, s.q0 * group + row0, min(a.shape.bm, s.qlen * group - row0));
+}
+
+// Item x of the grid, for up to 64 requests: every wave finds it by itself, a request a
+// lane.  The sum of the work (the key tiles of all blocks) gives the tiles to an item,
+// the running sum of the items the request that owns item x.  An item's first workgroup
+// fills its block's line of the table that the merge reads, and workgroups past the last
+// item the lines past the last block.
+constexpr int32_t PA_INLINE_SEQS = 64;
 __device__ __forceinline__ Item locate(const PagedArgs& a, int32_t x, bool writes_table) {
-  const int lane = threadIdx.x & 63;
-  const int32_t group = static_cast<int32_t>(a.group.d);
-  auto request = [&](int32_t b, bool& bad) {
-    bad = false;
-    PagedSeq s{0, 0, 0, 0, 0};
-    if (b < a.num_seqs)
-      s = paged_seq(a.qo_indptr[b], a.qo_indptr[b + 1], a.kv_indptr[b], a.kv_indptr[b + 1], a.last[b], a.tokens,
-                    a.num_indices, static_cast<int32_t>(a.ps.d), bad);
-    return s;
-  };
   bool bad;
-  PagedSeq s = request(lane, bad);
-  PagedSplit sp = paged_split(s, group, BM, a.window, a.sinks, KT);
+  const PagedSeq s = request(a, threadIdx.x & 63, bad);
+  const PagedSplit sp = paged_split(s, a.shape);
+  if (bad && x == 0 && writes_table) flag_status(a.status, BFA_STATUS_INDEX_OOB);
   int32_t per = INT_MAX;
-  if (a.split) {
-    int64_t total = static_cast<int64_t>(sp.blocks) * sp.tiles;
-    for (int32_t b = 64 + lane; b - lane < a.num_seqs; b += 64) {
-      bool ignored;
-      const PagedSplit q = paged_split(request(b, ignored), group, BM, a.window, a.sinks, KT);
-      total += static_cast<int64_t>(q.blocks) * q.tiles;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
-    per = paged_per_item(total, a.target, a.least);
-  }
+  if (a.split)
+    per = paged_per_item(__builtin_amdgcn_readlane(scan_lanes(paged_work(sp, a.shift)), 63), a.shift, a.target, a.least);
+  const int32_t chunks = sp.chunks(per), end = scan_lanes(paged_items(sp, per)), start = lane_before(end);
+  const uint64_t owner = __ballot(x >= start && x < end);
+  const int src = owner ? __builtin_ctzll(owner) : 63;
+  auto rd = [&](int32_t v) { return __builtin_amdgcn_readlane(v, src); };
   Item it{};
-  int32_t items = 0, blocks = 0;  // of the requests before
-  for (int32_t b = lane;; b += 64) {
-    if (b != lane) {
-      s = request(b, bad);
-      sp = paged_split(s, group, BM, a.window, a.sinks, KT);
-    }
-    if (bad && x == 0 && writes_table) flag_status(a.status, BFA_STATUS_INDEX_OOB);
-    const int32_t chunks = sp.chunks(per);
-    const int32_t mine = static_cast<int32_t>(min<int64_t>(static_cast<int64_t>(sp.blocks) * chunks, SCAN_MOST));
-    const int32_t end = scan_lanes(mine, lane), start = before(end, lane);
-    const int32_t bend = scan_lanes(sp.blocks, lane), bstart = before(bend, lane);
-    const uint64_t owner = __ballot(x - items >= start && x - items < end);
-    if (owner) {
-      const int src = __builtin_ctzll(owner);
-      auto rd = [&](int32_t v) { return __builtin_amdgcn_readlane(v, src); };
-      it.s = PagedSeq{rd(s.q0), rd(s.qlen), rd(s.page0), rd(s.npages), rd(s.kvlen)};
-      it.chunks = rd(chunks);
-      const int32_t in = x - items - rd(start);
-      it.block = in / it.chunks;
-      it.chunk = in - it.block * it.chunks;
-      it.index = x;
-      it.live = true;
-      // (read out here, where every lane is active: the compiler may compute what a lane
-      // read gives away under the branch that uses it)
-      const int32_t at = blocks + rd(bstart) + it.block;
-      if (a.split && writes_table && it.chunk == 0 && threadIdx.x == 0) {
-        const int32_t row0 = it.block * BM;
-        if (at < a.nblocks)
-          a.table[at] = make_int4(x, it.chunks, it.s.q0 * group + row0,
-                                  static_cast<int32_t>(min<int64_t>(BM, static_cast<int64_t>(it.s.qlen) * group - row0)));
-      }
-      return it;
-    }
-    items = min(items + __builtin_amdgcn_readlane(end, 63), SCAN_MOST);
-    blocks = min(blocks + __builtin_amdgcn_readlane(bend, 63), SCAN_MOST);
-    if (b - lane + 64 >= a.num_seqs) break;
+  if (owner) {
+    it.s = PagedSeq{rd(s.q0), rd(s.qlen), rd(s.page0), rd(s.npages), rd(s.kvlen)};
+    it.chunks = rd(chunks);
+    const int32_t in = x - rd(start);
+    it.block = it.chunks > 1 ? in / it.chunks : in;
+    it.chunk = in - it.block * it.chunks;
   }
-  if (a.split && writes_table && threadIdx.x == 0) {
-    const int64_t at = static_cast<int64_t>(blocks) + (x - items);
-    if (at < a.nblocks) a.table[at] = make_int4(0, 0, 0, 0);
+  if (a.split && writes_table) {
+    // (read out here, where every lane is active: the compiler may compute what a lane
+    // read gives away under the branch that uses it)
+    const int32_t bend = scan_lanes(sp.blocks);
+    const int32_t at = owner ? rd(lane_before(bend)) + it.block : rd(bend) + (x - rd(end));
+    if (threadIdx.x == 0 && it.chunk == 0 && at < a.nblocks)
+      a.table[at] = owner ? table_line(a, it.s, it.block, it.chunks, x) : make_int4(0, 0, 0, 0);
   }
   return it;
+}
+
+// The same for more requests, by one workgroup ahead of the others: all items, and the
+// table, 1024 requests at a time.  (512 requests of one key each: the items found by
+// every workgroup for itself TIME_INLINE, so TIME_PLAN.)
+__global__ __launch_bounds__(1024) void paged_plan_kernel(PagedArgs a) {
+  __shared__ int32_t item_end[1024], block_end[1024], wave_sum[2][16];
+  const int tid = threadIdx.x, wid = tid >> 6;
+  // sum of v over the workgroup up to and with this thread, and over all of it
+  auto scan = [&](int32_t v, int k, int32_t& all) {
+    int32_t end = scan_lanes(v);
+    if ((tid & 63) == 63) wave_sum[k][wid] = end;
+    __syncthreads();
+    int32_t before = 0;
+    all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wid) before = paged_add(before, wave_sum[k][w]);
+      all = paged_add(all, wave_sum[k][w]);
+    }
+    __syncthreads();
+    return paged_add(end, before);
+  };
+  int32_t per = INT_MAX;
+  if (a.split) {
+    int32_t work = 0, all;
+    for (int32_t b = tid; b < a.num_seqs; b += 1024) {
+      bool bad;
+      work = paged_add(work, paged_work(paged_split(request(a, b, bad), a.shape), a.shift));
+    }
+    scan(work, 0, all);
+    per = paged_per_item(all, a.shift, a.target, a.least);
+  }
+  int32_t items = 0, blocks = 0;  // of the requests before
+  for (int32_t b0 = 0; b0 < a.num_seqs; b0 += 1024) {
+    bool bad;
+    const PagedSplit sp = paged_split(request(a, b0 + tid, bad), a.shape);
+    if (bad) flag_status(a.status, BFA_STATUS_INDEX_OOB);
+    int32_t all_items, all_blocks;
+    item_end[tid] = scan(paged_items(sp, per), 0, all_items);
+    block_end[tid] = scan(sp.blocks, 1, all_blocks);
+    __syncthreads();
+    for (int32_t x = tid; x < all_items && items + x < a.items; x += 1024) {
+      int lo = 0, hi = 1023;  // the first request that ends past x
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (item_end[mid] > x) hi = mid;
+        else lo = mid + 1;
+      }
+      bool ignored;
+      const PagedSeq s = request(a, b0 + lo, ignored);
+      const int32_t chunks = paged_split(s, a.shape).chunks(per), in = x - (lo ? item_end[lo - 1] : 0);
+      const int32_t block = in / chunks, chunk = in - block * chunks;
+      a.plan[2 * (items + x)] = make_int4(s.q0, s.qlen, s.page0, s.npages);
+      a.plan[2 * (items + x) + 1] = make_int4(s.kvlen, block, chunk, chunks);
+      const int32_t at = paged_add(blocks, paged_add(lo ? block_end[lo - 1] : 0, block));
+      if (a.split && chunk == 0 && at < a.nblocks) a.table[at] = table_line(a, s, block, chunks, items + x);
+    }
+    items = paged_add(items, all_items);
+    blocks = paged_add(blocks, all_blocks);
+    __syncthreads();
+  }
+  for (int32_t x = items + tid; x < a.items; x += 1024) a.plan[2 * x + 1] = make_int4(0, 0, 0, 0);
+  if (a.split)
+    for (int32_t at = blocks + tid; at < a.nblocks; at += 1024) a.table[at] = make_int4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ Item find_item(const PagedArgs& a, int32_t x, bool writes_table) {
+  if (!a.plan) return locate(a, x, writes_table);
+  const int4 p = a.plan[2 * x], q = a.plan[2 * x + 1];
+  auto rd = [](int32_t v) { return __builtin_amdgcn_readfirstlane(v); };
+  return Item{PagedSeq{rd(p.x), rd(p.y), rd(p.z), rd(p.w), rd(q.x)}, rd(q.y), rd(q.z), rd(q.w)};
 }
 
 // The rows of a block: positions and query addresses.
@@ -396,7 +445,7 @@ template <int BM>
 __device__ __forceinline__ Rows block_rows(const PagedArgs& a, const Item& it) {
   Rows r;
   r.row0 = it.block * BM;
-  r.n = static_cast<int32_t>(min<int64_t>(BM, static_cast<int64_t>(it.s.qlen) * a.group.d - r.row0));
+  r.n = min(BM, it.s.qlen * static_cast<int32_t>(a.group.d) - r.row0);
   const int32_t base = it.s.kvlen - it.s.qlen;
   r.first = base + static_cast<int32_t>(a.group.div(r.row0));
   r.last = base + static_cast<int32_t>(a.group.div(r.row0 + r.n - 1));
@@ -501,7 +550,7 @@ __device__ __forceinline__ void poison(const PagedArgs& a, const PagedSeq& s, in
   const uint8_t* vbase = a.cache + h * a.c_sh + a.c_skv;
   for (int32_t i = i0; i < i1; i += step) {
     const int32_t key0 = kt.at(i) * KT;
-    if (!tile_edge(key0, KT, first, last, a.window, a.sinks)) continue;
+    if (!tile_edge(key0, KT, first, last, a.shape.window, a.sinks)) continue;
     for (int32_t key = key0; key < min(key0 + KT, s.kvlen); ++key) {
       const KeyRow kr = key_row<FP4>(a, s, key, key_entry(a, s, key));
       if (!kr.ok) continue;
@@ -538,7 +587,7 @@ __device__ __forceinline__ void poison(const PagedArgs& a, const PagedSeq& s, in
 // The next tile's rows are in flight during a tile's work, and the page ids of the
 // one after.  Bound by the cache's bytes.
 template <bool BF16, int D, bool FP4, bool P16>
-__global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, 3) void paged_decode_kernel(PagedArgs a) {
   constexpr int KT = 32, KC = KT / 16;
   constexpr int GK = D / 8, QJ = D / 32, OJ = D / 16;
   constexpr int VN = FP4 ? KT / 16 : KT * GK / 64;  // V loads of a lane: a quarter row of codes, or a granule
@@ -549,10 +598,11 @@ __global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(P
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t x = a.heads.div(blockIdx.x), h = blockIdx.x - x * a.hkv;
-  const Item it = locate<16, KT>(a, static_cast<int32_t>(x), h == 0);
-  if (!it.live) return;
+  const int32_t index = static_cast<int32_t>(x);
+  const Item it = find_item(a, index, h == 0);
+  if (it.chunks == 0) return;
   const Rows rows = block_rows<16>(a, it);
-  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
+  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.shape);
   const int32_t per = paged_even(kt.count, it.chunks);
   const int32_t i0 = min(it.chunk * per, kt.count), i1 = min(i0 + per, kt.count);
 
@@ -569,7 +619,7 @@ __global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(P
     for (int j = 0; j < QJ; ++j)
       qf[j] = query_words(a, qrow + (FP4 ? D / 4 * g4 + 8 * j : 32 * j + 8 * g4));
     hi[0] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
-    lo[0] = window_from(hi[0], a.window);
+    lo[0] = window_from(hi[0], a.shape.window);
   }
 
   float m[1] = {-INFINITY}, l[1] = {0.f};
@@ -622,7 +672,7 @@ __global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(P
     int32_t id = entry(i);
     for (; i < i1; i += 4) {
       const int32_t key0 = kt.at(i) * KT;
-      const bool edge = tile_edge(key0, KT, rows.first, rows.last, a.window, a.sinks);
+      const bool edge = tile_edge(key0, KT, rows.first, rows.last, a.shape.window, a.sinks);
       const int32_t id2 = entry(i + 4);
       const Keys keys(a, it.s, key0, id, lane);
       const Tile cur = issue(keys);
@@ -726,7 +776,7 @@ __global__ __launch_bounds__(256, FP4 && P16 ? 4 : 3) void paged_decode_kernel(P
           make_uint2(pa_pack<BF16>(acc[0].x * inv, acc[0].y * inv), pa_pack<BF16>(acc[0].z * inv, acc[0].w * inv));
     }
   } else {
-    const int64_t slot = (static_cast<int64_t>(it.index) * a.hkv + h) * 16 + r;
+    const int64_t slot = (static_cast<int64_t>(index) * a.hkv + h) * 16 + r;
     float4* dst = reinterpret_cast<float4*>(a.acc + slot * D) + D / 64 * (tid & 15);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) dst[c] = acc[c];
@@ -753,10 +803,11 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   const uint32_t x = a.heads.div(blockIdx.x), h = blockIdx.x - x * a.hkv;
   // the last blocks of a request see the most keys: they go first
   const int32_t grid_items = static_cast<int32_t>(a.heads.div(gridDim.x));
-  const Item it = locate<BM, KT>(a, grid_items - 1 - static_cast<int32_t>(x), h == 0);
-  if (!it.live) return;
+  const int32_t index = grid_items - 1 - static_cast<int32_t>(x);
+  const Item it = find_item(a, index, h == 0);
+  if (it.chunks == 0) return;
   const Rows rows = block_rows<BM>(a, it);
-  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.window, a.sinks, KT);
+  const KeyTiles kt = paged_key_tiles(rows.first, rows.last, it.s.kvlen, a.shape);
   const int32_t per = paged_even(kt.count, it.chunks);
   const int32_t i0 = min(it.chunk * per, kt.count), i1 = min(i0 + per, kt.count);
 
@@ -770,7 +821,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 #pragma unroll
     for (int j = 0; j < QJ; ++j) qf[rb][j] = query_words(a, qrow + 32 * j + 8 * g4);
     hi[rb] = it.s.kvlen - it.s.qlen + static_cast<int32_t>(t);
-    lo[rb] = window_from(hi[rb], a.window);
+    lo[rb] = window_from(hi[rb], a.shape.window);
   }
   // positions of this wave's first and last row (a wave without rows repeats the last)
   const int32_t base = it.s.kvlen - it.s.qlen;
@@ -888,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
     }
   };
   auto wg_edge = [&](int32_t i) {
-    return tile_edge(kt.at(i) * KT, KT, rows.first, rows.last, a.window, a.sinks);
+    return tile_edge(kt.at(i) * KT, KT, rows.first, rows.last, a.shape.window, a.sinks);
   };
   if (i0 < i1) {
     uint64_t exists, ahead;
@@ -915,7 +966,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
       id = id2;
       const int32_t key0 = kt.at(i) * KT;
       // (a wave skips a tile that none of its rows sees)
-      if (!idle && key0 <= wlast && (key0 + KT > window_from(wfirst, a.window) || key0 < a.sinks)) {
+      if (!idle && key0 <= wlast && (key0 + KT > window_from(wfirst, a.shape.window) || key0 < a.sinks)) {
         pa_f32x4_t sc[RB][KC];
 #pragma unroll
         for (int c = 0; c < KC; ++c)
@@ -930,7 +981,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) sc[rb][c] = pa_mfma<BF16>(kf, qf[rb][j], sc[rb][c]);
           }
-        if (tile_edge(key0, KT, wfirst, wlast, a.window, a.sinks) || exists != Keys::all())
+        if (tile_edge(key0, KT, wfirst, wlast, a.shape.window, a.sinks) || exists != Keys::all())
           hide<KC, RB>(sc, exists, key0, hi, lo, a.sinks, lane);
         attend<BF16, D, KC, RB>(sc, a.sl2, m, l, o, vbuf[b], lane);
       }
@@ -958,7 +1009,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
         *reinterpret_cast<uint2*>(orow + 16 * j) = make_uint2(pa_pack<BF16>(o[rb][j][0] * inv, o[rb][j][1] * inv),
                                                               pa_pack<BF16>(o[rb][j][2] * inv, o[rb][j][3] * inv));
     } else {
-      const int64_t slot = (static_cast<int64_t>(it.index) * a.hkv + h) * BM + r;
+      const int64_t slot = (static_cast<int64_t>(index) * a.hkv + h) * BM + r;
       float4* dst = reinterpret_cast<float4*>(a.acc + slot * D) + g4;
 #pragma unroll
       for (int j = 0; j < OJ; ++j) dst[4 * j] = make_float4(o[rb][j][0], o[rb][j][1], o[rb][j][2], o[rb][j][3]);
@@ -1038,9 +1089,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 // -------------------------------------------------------------------- plan
 struct PagedPlan {
   int bm, rb;                     // rows of a block; rb 0: the decode form
-  int32_t split, target, least, nblocks, items;
-  int64_t acc_bytes, ml_bytes, table_bytes;
-  int64_t total() const { return acc_bytes + ml_bytes + table_bytes; }
+  PagedShape shape;
+  int32_t split, target, least, shift, nblocks, items;
+  int64_t acc_bytes, ml_bytes, table_bytes, plan_bytes;
+  int64_t total() const { return acc_bytes + ml_bytes + table_bytes + plan_bytes; }
 };
 
 // The form follows the rows of an average request, and the items the workgroups that
@@ -1054,11 +1106,12 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
   if (forced == 16 || forced == 64 || forced == 128) p.rb = forced / 64;
   p.bm = p.rb == 0 ? 16 : 64 * p.rb;
   const int64_t kt = p.rb == 0 ? 32 : 64;
+  p.shape = paged_shape(p.bm, static_cast<int32_t>(group), static_cast<int32_t>(kt), static_cast<int32_t>(window),
+                        static_cast<int32_t>(sinks));
   p.nblocks = static_cast<int32_t>(std::min(rows, rows / p.bm + num_seqs));
   p.least = p.rb == 0 ? 4 : 2;
   const int64_t all = cdiv(num_indices * page_size, kt) + num_seqs;  // key tiles of all requests
-  int64_t most = all;                                               // of a block
-  if (window > 0) most = std::min(most, (window + p.bm / group + 2) / kt + 2 + sinks / kt + 1);
+  const int64_t most = std::min<int64_t>(all, p.shape.most);        // of a block
   const int wanted = tuning(BFA_TUNE_PAGED_WG);  // planner override
   int64_t wish = cdiv(wanted > 0 ? wanted : p.rb == 0 ? 2560 : 512, hkv);
   if (wanted <= 0) wish = std::max<int64_t>(wish - p.nblocks, cdiv(wish, 4));
@@ -1066,6 +1119,8 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
   p.split = most > p.least && (p.rb == 0 ? p.nblocks * hkv < 8192 : p.nblocks * hkv < 1024);
   if (wanted >= 0) p.split = wanted > 0 && most > p.least;
   p.items = p.nblocks + (p.split ? p.target : 0);
+  while (p.nblocks * ((most >> p.shift) + 1) > PAGED_MOST) ++p.shift;
+  if (num_seqs > PA_INLINE_SEQS) p.plan_bytes = static_cast<int64_t>(p.items) * 32;
   if (p.split) {
     const int64_t slots = static_cast<int64_t>(p.items) * hkv * p.bm;
     p.acc_bytes = slots * d * 4;
@@ -1173,16 +1228,19 @@ extern "C" int bfa_paged_attention(
   a.qand = scale == 0.f ? 0u : 0xffffffffu;
   a.qxor = scale < 0.f ? 0x80008000u : 0u;
   a.oscale = back;
-  a.window = static_cast<int32_t>(win); a.sinks = static_cast<int32_t>(snk);
+  a.shape = p.shape; a.sinks = static_cast<int32_t>(snk);
   a.out = static_cast<uint16_t*>(out); a.out_st = out_stride_token;
-  a.split = p.split; a.target = p.target; a.least = p.least; a.nblocks = p.nblocks;
+  a.split = p.split; a.target = p.target; a.least = p.least; a.shift = p.shift;
+  a.nblocks = p.nblocks; a.items = p.items;
   char* ws = static_cast<char*>(workspace);
   a.acc = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float*>(ws + p.acc_bytes);
   a.table = reinterpret_cast<int4*>(ws + p.acc_bytes + p.ml_bytes);
+  a.plan = p.plan_bytes ? reinterpret_cast<int4*>(ws + p.acc_bytes + p.ml_bytes + p.table_bytes) : nullptr;
   a.status = status;
   const hipStream_t s = as_stream(stream);
   const dim3 grid(static_cast<unsigned>(p.items * num_kv_heads));
+  if (a.plan) hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, s, a);
   const bool p16 = page_size % 16 == 0 && stride_slot / unit < (int64_t{1} << 23) && scale_stride_slot < (int64_t{1} << 27);
   auto launch = [&](auto bf, auto dd, auto four, auto by16) {
     constexpr bool B = decltype(bf)::value, F = decltype(four)::value, P = decltype(by16)::value;

@@ -60,38 +60,40 @@ _INTS = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 _FLOATS = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _ints(name: str, t: torch.Tensor):
-    """(contiguous one-dimensional tensor, its dtype's code)"""
+def _ints(name: str, t: torch.Tensor, n=None):
+    """(contiguous one-dimensional int32 or int64 tensor, of n elements if given; its code)"""
     code = _INTS.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-    if t.dim() != 1:
+    shape = t.shape
+    if len(shape) != 1:
         raise ValueError(f"{name} must be one-dimensional")
+    if n is not None and shape[0] != n:
+        raise IndexError(f"{shape[0]} {name.replace('_', ' ')} for {n} tokens")
     return (t if t.is_contiguous() else t.contiguous()), code
 
 
 def _tokens(cache, kv_indices, kv_indptr, batch_indices, positions, num_tokens):
     """Checked token addressing: the tensors, which the call must keep, and their
     entry-point arguments."""
-    positions, pos_code = _ints("positions", positions)
+    positions, pos_code = _ints("positions", positions, num_tokens)
     kv_indices, idx_code = _ints("kv_indices", kv_indices)
-    if positions.shape[0] != num_tokens:
-        raise IndexError(f"{positions.shape[0]} positions for {num_tokens} tokens")
-    if (kv_indptr is None) != (batch_indices is None):
-        raise ValueError("kv_indptr and batch_indices go together")
-    batched = (None, None, 0, 0)
-    if kv_indptr is not None:
-        batch_indices, code = _ints("batch_indices", batch_indices)
-        if batch_indices.shape[0] != num_tokens:
-            raise IndexError(f"{batch_indices.shape[0]} batch indices for {num_tokens} tokens")
-        if kv_indptr.dtype != torch.int32 or kv_indptr.dim() != 1 or kv_indptr.shape[0] < 1:
-            raise TypeError("kv_indptr must be a one-dimensional int32 tensor")
-        kv_indptr = kv_indptr if kv_indptr.is_contiguous() else kv_indptr.contiguous()
-        batched = (kv_indptr.data_ptr(), batch_indices.data_ptr(), code, kv_indptr.shape[0] - 1)
     if cache.page_size == 0 and num_tokens:
         raise ValueError("the cache's pages have no slots")
-    keep = (positions, kv_indices, kv_indptr, batch_indices)
-    return keep, (kv_indices.data_ptr(), idx_code, kv_indices.shape[0], *batched, positions.data_ptr(), pos_code)
+    if kv_indptr is None and batch_indices is None:
+        return (positions, kv_indices, None, None), (kv_indices.data_ptr(), idx_code, kv_indices.shape[0], None, None, 0, 0,
+                                                     positions.data_ptr(), pos_code)
+    if kv_indptr is None or batch_indices is None:
+        raise ValueError("kv_indptr and batch_indices go together")
+    batch_indices, code = _ints("batch_indices", batch_indices, num_tokens)
+    shape = kv_indptr.shape
+    if kv_indptr.dtype != torch.int32 or len(shape) != 1 or shape[0] < 1:
+        raise TypeError("kv_indptr must be a one-dimensional int32 tensor")
+    if not kv_indptr.is_contiguous():
+        kv_indptr = kv_indptr.contiguous()
+    return (positions, kv_indices, kv_indptr, batch_indices), (
+        kv_indices.data_ptr(), idx_code, kv_indices.shape[0], kv_indptr.data_ptr(), batch_indices.data_ptr(), code,
+        shape[0] - 1, positions.data_ptr(), pos_code)
 
 
 def append_paged_kv_fp4(
@@ -128,13 +130,9 @@ def append_paged_kv_fp4(
     dev = _lib.require_device(k, v, cache.codes, cache.scales, *keep)
     if tokens == 0:
         return
-    with _lib.on_device(dev):
-        rc = _lib.entry("bfa_append_paged_kv_fp4")(
-            k.data_ptr(), v.data_ptr(), code, tokens, heads, dim, ks[0], ks[1], vs[0], vs[1], cache.codes.data_ptr(),
-            cache.scales.data_ptr(), cache.num_pages, cache.page_size, *cache.strides, *where,
-            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
-    if rc < 0:
-        _lib.raise_error(rc)
+    _lib.launch(_lib.entry("bfa_append_paged_kv_fp4"), dev, k.data_ptr(), v.data_ptr(), code, tokens, heads, dim, ks[0],
+                ks[1], vs[0], vs[1], cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, cache.page_size,
+                *cache.strides, *where)
 
 
 def gather_paged_kv_fp4(
@@ -159,10 +157,6 @@ def gather_paged_kv_fp4(
     k, v = torch.empty((2, tokens, heads, dim), dtype=dtype, device=dev).unbind()
     if tokens == 0:
         return k, v
-    with _lib.on_device(dev):
-        rc = _lib.entry("bfa_gather_paged_kv_fp4")(
-            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, cache.page_size, heads, dim, *cache.strides,
-            *where, tokens, k.data_ptr(), v.data_ptr(), code, _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
-    if rc < 0:
-        _lib.raise_error(rc)
+    _lib.launch(_lib.entry("bfa_gather_paged_kv_fp4"), dev, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages,
+                cache.page_size, heads, dim, *cache.strides, *where, tokens, k.data_ptr(), v.data_ptr(), code)
     return k, v

@@ -50,40 +50,46 @@ def build_paged_kv_batch(
     append of a padded batch pass the live tokens' slices to ``append_paged_kv_batch``
     (it takes request -1 for an error); ``append_paged_kv_fp4`` skips padding itself.
     """
-    if page_tables.dim() != 2:
+    shape = page_tables.shape
+    if len(shape) != 2:
         raise ValueError("page_tables must be [requests, max_pages]")
-    seqs, width = page_tables.shape
-    codes = []
-    for name, t, dims in (("seq_lens", seq_lens, 1), ("query_lens", query_lens, 1), ("page_tables", page_tables, 2)):
-        if t.dim() != dims or t.shape[0] != seqs:
-            raise ValueError(f"{name} of shape {tuple(t.shape)} for {seqs} requests")
-        code = _INTS.get(t.dtype)
-        if code is None:
-            raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-        codes.append(code)
+    seqs, width = shape
+    if seq_lens.shape != (seqs,) or query_lens.shape != (seqs,):
+        name, t = ("seq_lens", seq_lens) if seq_lens.shape != (seqs,) else ("query_lens", query_lens)
+        raise ValueError(f"{name} of shape {tuple(t.shape)} for {seqs} requests")
+    table_code, seq_code, query_code = _INTS.get(page_tables.dtype), _INTS.get(seq_lens.dtype), _INTS.get(query_lens.dtype)
+    if table_code is None or seq_code is None or query_code is None:
+        raise TypeError("page_tables, seq_lens and query_lens must be int32 or int64 "
+                        f"(got {page_tables.dtype}, {seq_lens.dtype} and {query_lens.dtype})")
     if page_size <= 0:
         raise ValueError("page_size must be positive")
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    if width and page_tables.stride(1) != 1:
+    row, column = page_tables.stride()
+    if column != 1 and width:
         page_tables = page_tables.contiguous()
-    seq_lens, query_lens = seq_lens.contiguous(), query_lens.contiguous()
+        row = width
+    if not seq_lens.is_contiguous():
+        seq_lens = seq_lens.contiguous()
+    if not query_lens.is_contiguous():
+        query_lens = query_lens.contiguous()
     dev = _lib.require_device(page_tables, seq_lens, query_lens)
-    sizes = (seqs + 1, seqs + 1, seqs * width, seqs, num_tokens, num_tokens, num_tokens)
+    entries = seqs * width
     if out is None:
-        # two allocations for the seven (one of 1.4 us each otherwise)
-        out = PagedKVBatch(*torch.empty(sum(sizes[:5]), dtype=torch.int32, device=dev).split_with_sizes(sizes[:5]),
-                           *torch.empty(2, num_tokens, dtype=torch.int64, device=dev).unbind())
+        # two allocations for the seven tensors
+        words = torch.empty(2 * seqs + 2 + entries + seqs + num_tokens, dtype=torch.int32, device=dev)
+        qo, kv, idx, last, owner = words.split_with_sizes((seqs + 1, seqs + 1, entries, seqs, num_tokens))
+        positions, slots = torch.empty((2, num_tokens), dtype=torch.int64, device=dev).unbind()
+        out = PagedKVBatch(qo, kv, idx, last, owner, positions, slots)
     else:
+        sizes = (seqs + 1, seqs + 1, entries, seqs, num_tokens, num_tokens, num_tokens)
         for name, t, n, d in zip(out._fields, out, sizes, _DTYPES):
             if t.dtype != d or tuple(t.shape) != (n,) or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be a contiguous {d} tensor of {n} elements")
         _lib.require_device(page_tables, *out)
-    with _lib.on_device(dev):
-        rc = _lib.entry("bfa_build_paged_kv_batch")(
-            page_tables.data_ptr(), codes[2], seqs, width, page_tables.stride(0), seq_lens.data_ptr(), codes[0],
-            query_lens.data_ptr(), codes[1], int(page_size), num_tokens, seqs * width, *[t.data_ptr() for t in out],
-            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
-    if rc < 0:
-        _lib.raise_error(rc)
+        qo, kv, idx, last, owner, positions, slots = out
+    _lib.launch(_lib.entry("bfa_build_paged_kv_batch"), dev, page_tables.data_ptr(), table_code, seqs, width, row,
+                seq_lens.data_ptr(), seq_code, query_lens.data_ptr(), query_code, page_size, num_tokens, entries,
+                qo.data_ptr(), kv.data_ptr(), idx.data_ptr(), last.data_ptr(), owner.data_ptr(), positions.data_ptr(),
+                slots.data_ptr())
     return out

@@ -25,10 +25,7 @@ def _strides(t: torch.Tensor, unit: int):
     aligned; None if they are not.  0 for a dimension of one element, whose stride means
     nothing, where it is not such a multiple."""
     st = t.stride()
-    bits = 0
-    for s in st[:-1]:
-        bits |= s
-    if bits % unit:
+    if (st[0] | st[1] | (0 if len(st) < 4 else st[2] | st[3])) % unit:
         st = tuple(0 if n == 1 else s for n, s in zip(t.shape[:-1], st)) + st[-1:]
         if any(s % unit for s in st[:-1]):
             return None
@@ -112,16 +109,20 @@ def paged_attention(
         raise ValueError("window must be at least 1 (None for no window)")
     if num_sinks < 0:
         raise ValueError("num_sinks must not be negative")
-    if (kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_last_page_len.dtype != torch.int32
-            or qo_indptr.dtype != torch.int32 or kv_indices.dim() != 1 or kv_indptr.dim() != 1
-            or kv_last_page_len.dim() != 1 or qo_indptr.dim() != 1):
+    indices_shape, requests = kv_indices.shape, kv_last_page_len.shape
+    i32 = torch.int32
+    if (kv_indices.dtype != i32 or kv_indptr.dtype != i32 or kv_last_page_len.dtype != i32 or qo_indptr.dtype != i32
+            or len(indices_shape) != 1 or len(requests) != 1):
         raise TypeError("kv_indices, kv_indptr, kv_last_page_len and qo_indptr must be one-dimensional int32 tensors")
-    seqs, num_indices = kv_last_page_len.shape[0], kv_indices.shape[0]
-    if kv_indptr.shape[0] != seqs + 1 or qo_indptr.shape[0] != seqs + 1:
-        name, t = ("kv_indptr", kv_indptr) if kv_indptr.shape[0] != seqs + 1 else ("qo_indptr", qo_indptr)
-        raise ValueError(f"{name} has {t.shape[0]} elements, for {seqs} requests {seqs + 1} are needed")
-    kv_indices, kv_indptr = kv_indices.contiguous(), kv_indptr.contiguous()
-    kv_last_page_len, qo_indptr = kv_last_page_len.contiguous(), qo_indptr.contiguous()
+    seqs, num_indices = requests[0], indices_shape[0]
+    ends = (seqs + 1,)
+    if kv_indptr.shape != ends or qo_indptr.shape != ends:
+        name, t = ("kv_indptr", kv_indptr) if kv_indptr.shape != ends else ("qo_indptr", qo_indptr)
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, for {seqs} requests {seqs + 1} elements are needed")
+    if not (kv_indices.is_contiguous() and kv_indptr.is_contiguous() and kv_last_page_len.is_contiguous()
+            and qo_indptr.is_contiguous()):
+        kv_indices, kv_indptr = kv_indices.contiguous(), kv_indptr.contiguous()
+        kv_last_page_len, qo_indptr = kv_last_page_len.contiguous(), qo_indptr.contiguous()
     qs = _strides(query, 8)
     if qs is None:
         query = query.clone(memory_format=torch.contiguous_format)
@@ -141,14 +142,12 @@ def paged_attention(
     size = _lib.entry("bfa_paged_attention_workspace_size")(tokens, seqs, hq, hkv, dim, num_indices, slots, window, num_sinks,
                                                             cache_code)
     ws = _lib.scratch(dev)
-    with _lib.on_device(dev), ws.lock:
-        ws.reserve(size)
-        rc = _lib.entry("bfa_paged_attention")(
-            query.data_ptr(), code, tokens, hq, qs[0], qs[1], data.data_ptr(), cache_code, pages, hkv, slots, dim, st[0],
-            st[1], st[h], st[s], None if scales is None else scales.data_ptr(), *sst, kv_indices.data_ptr(), num_indices,
-            kv_indptr.data_ptr(), kv_last_page_len.data_ptr(), qo_indptr.data_ptr(), seqs,
-            dim ** -0.5 if scale is None else float(scale), window, num_sinks, out.data_ptr(), row, ws.ptr, ws.size,
-            _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
-    if rc < 0:
-        _lib.raise_error(rc)
+    with ws.lock:
+        if ws.size < size or ws.buf is None:
+            ws.reserve(size)
+        _lib.launch(_lib.entry("bfa_paged_attention"), dev, query.data_ptr(), code, tokens, hq, qs[0], qs[1], data.data_ptr(),
+                    cache_code, pages, hkv, slots, dim, st[0], st[1], st[h], st[s],
+                    None if scales is None else scales.data_ptr(), *sst, kv_indices.data_ptr(), num_indices,
+                    kv_indptr.data_ptr(), kv_last_page_len.data_ptr(), qo_indptr.data_ptr(), seqs,
+                    dim ** -0.5 if scale is None else scale, window, num_sinks, out.data_ptr(), row, ws.ptr, ws.size)
     return out

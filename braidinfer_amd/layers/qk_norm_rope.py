@@ -47,39 +47,38 @@ def qk_norm_rope(
         raise TypeError(f"query and key must be bf16, fp16 or fp32, not {query.dtype}")
     q, q_heads, q_token, q_head = _rows("query", query, tokens, dim)
     k, k_heads, k_token, k_head = _rows("key", key, tokens, dim)
-    w_code = None
-    ptrs = []
-    for w in (q_norm_weight, k_norm_weight):
-        if w is None:
-            ptrs.append((None, None))
-            continue
-        if w.numel() != dim:
-            raise ValueError(f"norm weights must have head_dim = {dim} elements")
-        c = _FLOATS.get(w.dtype)
-        if c is None or w_code not in (None, c):
+    qw, qw_ptr, w_code = _weight(q_norm_weight, dim)
+    kw, kw_ptr, k_code = _weight(k_norm_weight, dim)
+    if k_code != w_code:
+        if qw is not None and kw is not None:
             raise TypeError("norm weights must share a dtype: bf16, fp16 or fp32")
-        w_code = c
-        if not w.is_contiguous():
-            w = w.detach().contiguous()
-        ptrs.append((w, w.data_ptr()))
-    (qw, qw_ptr), (kw, kw_ptr) = ptrs
+        w_code = w_code if kw is None else k_code
     if not positions.is_contiguous():
         positions = positions.contiguous()
     if not cos_sin_cache.is_contiguous():
         cos_sin_cache = cos_sin_cache.contiguous()
     dev = _lib.require_device(q, k, positions, cos_sin_cache, qw, kw)
     q_out = torch.empty(query.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(key.shape, dtype=k.dtype, device=dev)
-    if tokens == 0:
-        return q_out, k_out
-    with _lib.on_device(dev):
-        rc = _lib.entry("bfa_qk_norm_rope")(
-            q.data_ptr(), q_heads, q_token, q_head, q_out.data_ptr(), k.data_ptr(), k_heads, k_token, k_head,
-            k_out.data_ptr(), code, tokens, dim, qw_ptr, kw_ptr, w_code or 0, float(eps), positions.data_ptr(), pos_code,
-            cos_sin_cache.data_ptr(), max_position, _lib.status_word(dev).data_ptr(), _lib.stream_of(dev))
-    if rc < 0:
-        _lib.raise_error(rc)
+    k_out = torch.empty(key.shape, dtype=q.dtype, device=dev)
+    if tokens:
+        _lib.launch(_lib.entry("bfa_qk_norm_rope"), dev, q.data_ptr(), q_heads, q_token, q_head, q_out.data_ptr(),
+                    k.data_ptr(), k_heads, k_token, k_head, k_out.data_ptr(), code, tokens, dim, qw_ptr, kw_ptr, w_code, eps,
+                    positions.data_ptr(), pos_code, cos_sin_cache.data_ptr(), max_position)
     return q_out, k_out
+
+
+def _weight(w: torch.Tensor | None, dim: int):
+    """(contiguous weight, its address, its dtype's code)"""
+    if w is None:
+        return None, None, 0
+    if w.numel() != dim:
+        raise ValueError(f"norm weights must have head_dim = {dim} elements")
+    code = _FLOATS.get(w.dtype)
+    if code is None:
+        raise TypeError("norm weights must share a dtype: bf16, fp16 or fp32")
+    if not w.is_contiguous():
+        w = w.detach().contiguous()
+    return w, w.data_ptr(), code
 
 
 _INTS = {torch.int32: _lib.I32, torch.int64: _lib.I64}
@@ -90,11 +89,14 @@ def _rows(name: str, x: torch.Tensor, tokens: int, dim: int):
     """(x with unit stride along a head's row, heads, token stride, head stride)"""
     shape = x.shape
     if len(shape) == 2 and shape[0] == tokens and shape[1] % dim == 0:
-        if x.stride(1) != 1:
+        token, last = x.stride()
+        if last != 1:
             x = x.contiguous()
-        return x, shape[1] // dim, x.stride(0), dim
+            token = shape[1]
+        return x, shape[1] // dim, token, dim
     if len(shape) == 3 and shape[0] == tokens and shape[2] == dim:
         if x.stride(2) != 1:
             x = x.contiguous()
-        return x, shape[1], x.stride(0), x.stride(1)
+        token, head, _ = x.stride()
+        return x, shape[1], token, head
     raise ValueError(f"{name} of shape {tuple(shape)} is not [{tokens}, heads * {dim}] or [{tokens}, heads, {dim}]")

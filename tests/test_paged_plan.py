@@ -23,19 +23,22 @@ int seq(const int* in, long long tokens, long long indices, int ps, int* out) {
 }
 long long page(long long id, long long pages) { return paged_page(id, pages); }
 int tiles(int first, int last, int kvlen, int window, int sinks, int tile, int* out) {
-  KeyTiles k = paged_key_tiles(first, last, kvlen, window, sinks, tile);
+  KeyTiles k = paged_key_tiles(first, last, kvlen, paged_shape(16, 1, tile, window, sinks));
   for (int i = 0; i < k.count && i < 4096; ++i) out[i] = k.at(i);
   return k.count;
 }
 int split(int qlen, int kvlen, int group, int bm, int window, int sinks, int tile, int* blocks) {
   PagedSeq s{0, qlen, 0, 0, kvlen};
-  PagedSplit p = paged_split(s, group, bm, window, sinks, tile);
+  PagedSplit p = paged_split(s, paged_shape(bm, group, tile, window, sinks));
   *blocks = p.blocks;
   return p.tiles;
 }
 int chunks(int blocks, int tiles, int per) { return PagedSplit{blocks, tiles}.chunks(per); }
 int even(int tiles, int chunks) { return paged_even(tiles, chunks); }
-int per_item(long long total, int target, int least) { return paged_per_item(total, target, least); }
+int work(int blocks, int tiles, int shift) { return paged_work(PagedSplit{blocks, tiles}, shift); }
+int items(int blocks, int tiles, int per) { return paged_items(PagedSplit{blocks, tiles}, per); }
+int add(int a, int b) { return paged_add(a, b); }
+int per_item(int work, int shift, int target, int least) { return paged_per_item(work, shift, target, least); }
 }
 """
 
@@ -53,7 +56,6 @@ def lib(tmp_path_factory):
     lib.page.restype = ctypes.c_longlong
     lib.page.argtypes = [ctypes.c_longlong] * 2
     lib.seq.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]
-    lib.per_item.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     return lib
 
 
@@ -128,7 +130,7 @@ def test_items_cover_every_block(lib):
         for _ in range(rng.randint(1, 6)):
             kvlen = rng.randint(0, 700)
             requests.append((rng.randint(0, min(kvlen + 2, 90)), kvlen))
-        total, plans = 0, []
+        plans, shift = [], rng.choice([0, 0, 1, 3])
         for qlen, kvlen in requests:
             blocks = ctypes.c_int()
             tiles = lib.split(qlen, kvlen, group, bm, window, sinks, tile, ctypes.byref(blocks))
@@ -137,18 +139,28 @@ def test_items_cover_every_block(lib):
                 r0, r1 = b * bm, min((b + 1) * bm, qlen * group) - 1
                 base = kvlen - qlen
                 assert len(key_tiles(lib, base + r0 // group, base + r1 // group, kvlen, window, sinks, tile)) <= tiles
-            total += blocks.value * tiles
             plans.append((blocks.value, tiles))
+        total = 0
+        for b, t in plans:
+            total = lib.add(total, lib.work(b, t, shift))
         target, least = rng.randint(1, 40), rng.choice([1, 2, 4])
-        per = lib.per_item(total, target, least)
-        items = sum(b * lib.chunks(b, t, per) for b, t in plans)
+        per = lib.per_item(total, shift, target, least)
+        items = sum(lib.items(b, t, per) for b, t in plans)
         assert per >= least and items <= target + sum(b for b, _ in plans)
         assert all(lib.chunks(b, t, per) * per >= t for b, t in plans)
-        rows = sum(q for q, _ in requests) * group
-        assert sum(b for b, _ in plans) <= min(rows, rows // bm + len(requests))
         for _, t in plans:
             c = lib.chunks(1, t, per)
             assert t <= lib.even(t, c) * c and (c == 1 or lib.even(t, c) <= per)
+        rows = sum(q for q, _ in requests) * group
+        assert sum(b for b, _ in plans) <= min(rows, rows // bm + len(requests))
     assert lib.even(0, 1) == 0 and lib.even(2 ** 31 - 1, 1) == 2 ** 31 - 1 and lib.even(7, 3) == 3
     assert lib.chunks(1, 0, 4) == 1 and lib.chunks(1, 2 ** 31 - 1, 2 ** 31 - 1) == 1
-    assert lib.per_item(2 ** 60, 1, 2) == 0x3fffffff
+
+
+def test_sums_of_broken_requests_do_not_overflow(lib):
+    most = 0x3fffffff
+    assert lib.work(2 ** 27, 2 ** 26, 0) == most and lib.work(8192, 2 ** 26, 10) == 8192 * 2 ** 16
+    assert lib.items(2 ** 27, 2 ** 26, 1) == most and lib.add(most, most) == most and lib.add(most, 5) == most
+    assert lib.per_item(most, 0, 1, 2) == most and lib.per_item(most, 20, 1, 2) == most
+    assert lib.per_item(0, 0, 300, 4) == 4 and lib.per_item(8192 * 2 ** 16, 10, 320, 4) == most  # (-> 1.7e9 tiles)
+    assert lib.per_item(2 ** 20, 10, 320, 4) == -(-2 ** 20 // 320) * 1024
