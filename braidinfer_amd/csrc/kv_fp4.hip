@@ -15,6 +15,8 @@
 // Codes: [pages, 2, heads, slots, D / 2], scales: [pages, 2, heads, slots, D / 32] bytes
 // (any strides but the last).  4 lanes take a block, 8 elements each.  Bound by the
 // bytes: 16-bit k and v in, 4.25 bits an element out.
+#include <type_traits>
+
 #include "bfa_append.h"
 #include "bfa_device.h"
 #include "bfa_host.h"
@@ -33,58 +35,60 @@ struct Fp4Args {
   FastDiv per_token;  // 2 * heads * D / 8
 };
 
-// one lane's place: token, K or V, head, element; false past the end
+// A workgroup takes 256 N chunks of 8 elements, N to a lane, in order of token, K or V,
+// head, element.  Its first lanes find where its tokens go (three dependent reads a
+// token, while the elements' loads are in flight) and leave that in the LDS: with each
+// lane finding its own token's place, one chunk a lane, 6000 tokens of 8 x 128 took
+// 14.8 us to append, the loads' latency and that one's after another.
+constexpr int FP4_TOKENS = 256 * 4 / 8 + 2;  // of a workgroup at most: 8 chunks a token at least
+struct Fp4Place {
+  int64_t codes, scales;  // byte offsets of the token's slot, -1: it has none
+};
+__device__ __forceinline__ void fp4_places(const Fp4Args& f, int64_t t0, int64_t t1, Fp4Place* places) {
+  const AppendArgs& a = f.a;
+  const int64_t t = t0 + threadIdx.x;
+  if (t <= t1) {
+    Fp4Place p{-1, -1};
+    const AppendKey key = append_key(a, t);
+    if (!(a.indptr && key.seq == -1)) {  // (request -1 is padding, which is no error)
+      int64_t page = 0, slot = 0;
+      const int bad = append_resolve(a, key, page, slot);
+      if (bad) flag_status(a.status, bad);
+      else p = Fp4Place{page * a.c_sp + slot * a.c_ss, page * f.s_sp + slot * f.s_ss};
+    }
+    places[threadIdx.x] = p;
+  }
+  __syncthreads();
+}
+
+// chunk i: its token, K or V, head and first element
 struct Fp4Item {
   int64_t t;
   uint32_t kv, h, e;
 };
-__device__ __forceinline__ bool fp4_item(const Fp4Args& f, Fp4Item& it) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= f.tokens * f.per_token.d) return false;  // whole groups of 4 lanes
-  it.t = f.per_token.div(static_cast<uint32_t>(i));
-  const uint32_t r = static_cast<uint32_t>(i) - static_cast<uint32_t>(it.t) * f.per_token.d;
+__device__ __forceinline__ Fp4Item fp4_item(const Fp4Args& f, uint32_t i) {
+  Fp4Item it;
+  it.t = f.per_token.div(i);
+  const uint32_t r = i - static_cast<uint32_t>(it.t) * f.per_token.d;
   it.kv = f.a.chunks_per_kv.div(r);
   const uint32_t q = r - it.kv * f.a.chunks_per_kv.d;
   it.h = f.a.chunks_per_head.div(q);
   it.e = (q - it.h * f.a.chunks_per_head.d) * 8;
-  return true;
+  return it;
 }
 
-// Where a token's rows are; false (the reason flagged) where it has none.  A token of
-// request -1 is padding, which is no error.
-__device__ __forceinline__ bool fp4_target(const Fp4Args& f, int64_t t, int64_t& page, int64_t& slot) {
-  const AppendKey key = append_key(f.a, t);
-  if (f.a.indptr && key.seq == -1) return false;
-  const int bad = append_resolve(f.a, key, page, slot);
-  if (bad && (threadIdx.x & 3) == 0) flag_status(f.a.status, bad);
-  return bad == 0;
-}
-
-template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void kv_fp4_append_kernel(Fp4Args f) {
-  using T = typename Elem<DT>::T;
-  const AppendArgs& a = f.a;
-  Fp4Item it;
-  if (!fp4_item(f, it)) return;
-  const T* src = it.kv == 0 ? static_cast<const T*>(a.k) + it.t * a.k_st + it.h * a.k_sh
-                            : static_cast<const T*>(a.v) + it.t * a.v_st + it.h * a.v_sh;
-  float x[8];
-  if constexpr (VEC) {
-    load8_nt<DT>(src + it.e, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<DT>::to_f32(src[it.e + i]);
-  }
+// 8 elements as codes, with the scale byte of their block, which 4 lanes share
+__device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], uint32_t& byte) {
   // largest magnitude of the block, as bits (a NaN's are above an infinity's)
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-  most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 1)));
-  most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 2)));
+  most = max(most, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(most), 0xB1, 0xF, 0xF, false)));
+  most = max(most, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(most), 0x4E, 0xF, 0xF, false)));
   // 1.m x 2^E stays within 6 x 2^e = 1.5 x 2^(e + 2) with e = E - 2, or E - 1 where 1.m > 1.5
   const int e = max(static_cast<int>(most >> 23) - 129 + ((most & 0x7fffffu) > 0x400000u ? 1 : 0), -126);
   const bool finite = most < 0x7f800000u;
-  const uint32_t byte = finite ? static_cast<uint32_t>(e + 127) : 255u;
+  byte = finite ? static_cast<uint32_t>(e + 127) : 255u;
   const float scale = __uint_as_float(byte << 23);
   uint32_t w = 0;
   if (finite) {
@@ -93,12 +97,42 @@ __global__ __launch_bounds__(256) void kv_fp4_append_kernel(Fp4Args f) {
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
   }
-  int64_t page = 0, slot = 0;
-  if (!fp4_target(f, it.t, page, slot)) return;
-  uint8_t* dst = static_cast<uint8_t*>(a.cache) + page * a.c_sp + it.kv * a.c_skv + it.h * a.c_sh + slot * a.c_ss;
-  *reinterpret_cast<uint32_t*>(dst + it.e / 2) = w;
-  if ((threadIdx.x & 3) == 0)
-    f.scales[page * f.s_sp + it.kv * f.s_skv + it.h * f.s_sh + slot * f.s_ss + it.e / 32] = static_cast<uint8_t>(byte);
+  return w;
+}
+
+template <int DT, bool VEC, int N>
+__global__ __launch_bounds__(256) void kv_fp4_append_kernel(Fp4Args f) {
+  using T = typename Elem<DT>::T;
+  const AppendArgs& a = f.a;
+  __shared__ Fp4Place places[FP4_TOKENS];
+  const uint32_t total = static_cast<uint32_t>(f.tokens) * f.per_token.d, i0 = blockIdx.x * 256u * N;
+  const uint32_t last = min(i0 + 256u * N, total) - 1;
+  Fp4Item it[N];
+  float x[N][8];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {  // (a lane past the end takes the last chunk, and stores nothing)
+    it[n] = fp4_item(f, min(i0 + 256u * n + threadIdx.x, last));
+    const T* src = it[n].kv == 0 ? static_cast<const T*>(a.k) + it[n].t * a.k_st + it[n].h * a.k_sh
+                                 : static_cast<const T*>(a.v) + it[n].t * a.v_st + it[n].h * a.v_sh;
+    if constexpr (VEC) {
+      load8_nt<DT>(src + it[n].e, x[n]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[n][i] = Elem<DT>::to_f32(src[it[n].e + i]);
+    }
+  }
+  const int64_t t0 = f.per_token.div(i0);
+  fp4_places(f, t0, f.per_token.div(last), places);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t byte;
+    const uint32_t w = fp4_codes(x[n], byte);
+    const Fp4Place p = places[it[n].t - t0];
+    if (i0 + 256u * n + threadIdx.x > last || p.codes < 0) continue;
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.cache) + p.codes + it[n].kv * a.c_skv + it[n].h * a.c_sh + it[n].e / 2) = w;
+    if ((threadIdx.x & 3) == 0)
+      f.scales[p.scales + it[n].kv * f.s_skv + it[n].h * f.s_sh + it[n].e / 32] = static_cast<uint8_t>(byte);
+  }
 }
 
 // 8 codes and their scale as fp32, exactly
@@ -111,21 +145,36 @@ __device__ __forceinline__ void fp4_values(uint32_t w, uint32_t byte, float (&x)
   x[4] = v2.x; x[5] = v2.y; x[6] = v3.x; x[7] = v3.y;
 }
 
-template <int DT>
+template <int DT, int N>
 __global__ __launch_bounds__(256) void kv_fp4_gather_kernel(Fp4Args f) {
   using T = typename Elem<DT>::T;
   const AppendArgs& a = f.a;
-  Fp4Item it;
-  if (!fp4_item(f, it)) return;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int64_t page = 0, slot = 0;
-  if (fp4_target(f, it.t, page, slot)) {
-    const uint8_t* src = static_cast<const uint8_t*>(a.cache) + page * a.c_sp + it.kv * a.c_skv + it.h * a.c_sh + slot * a.c_ss;
-    const uint32_t byte = f.scales[page * f.s_sp + it.kv * f.s_skv + it.h * f.s_sh + slot * f.s_ss + it.e / 32];
-    fp4_values(*reinterpret_cast<const uint32_t*>(src + it.e / 2), byte, x);
+  __shared__ Fp4Place places[FP4_TOKENS];
+  const uint32_t total = static_cast<uint32_t>(f.tokens) * f.per_token.d, i0 = blockIdx.x * 256u * N;
+  const uint32_t last = min(i0 + 256u * N, total) - 1;
+  const int64_t t0 = f.per_token.div(i0);
+  fp4_places(f, t0, f.per_token.div(last), places);
+  Fp4Item it[N];
+  uint32_t w[N], byte[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    it[n] = fp4_item(f, min(i0 + 256u * n + threadIdx.x, last));
+    const Fp4Place p = places[it[n].t - t0];
+    w[n] = byte[n] = 0;  // (no place: zeros)
+    if (p.codes >= 0) {
+      w[n] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.cache) + p.codes + it[n].kv * a.c_skv +
+                                                it[n].h * a.c_sh + it[n].e / 2);
+      byte[n] = f.scales[p.scales + it[n].kv * f.s_skv + it[n].h * f.s_sh + it[n].e / 32];
+    }
   }
-  T* dst = static_cast<T*>(it.kv == 0 ? f.k_out : f.v_out) + (it.t * a.heads + it.h) * a.head_dim + it.e;
-  store8<DT>(dst, x);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (i0 + 256u * n + threadIdx.x > last) continue;
+    float x[8];
+    fp4_values(w[n], byte[n], x);
+    T* dst = static_cast<T*>(it[n].kv == 0 ? f.k_out : f.v_out) + (it[n].t * a.heads + it[n].h) * a.head_dim + it[n].e;
+    store8<DT>(dst, x);
+  }
 }
 
 // Checks and fills what the append and the gather share.
@@ -164,7 +213,13 @@ static int fp4_args(const char* what, const void* codes, const void* scales, int
   return BFA_OK;
 }
 
-static dim3 fp4_grid(const Fp4Args& f) { return dim3(static_cast<unsigned>(cdiv(f.tokens * f.per_token.d, 256))); }
+// 4 chunks a lane where that leaves at least two workgroups a CU (64 tokens of 8 x 128,
+// 64 workgroups of one chunk a lane, are latency: 3.8 us; 6000 tokens TIME_N1 us with one
+// chunk, TIME_N4 us with four)
+static bool fp4_many(const Fp4Args& f) { return f.tokens * f.per_token.d >= int64_t{512} * 1024; }
+static dim3 fp4_grid(const Fp4Args& f, int n) {
+  return dim3(static_cast<unsigned>(cdiv(f.tokens * f.per_token.d, 256 * n)));
+}
 
 }  // namespace bfa
 
@@ -199,8 +254,9 @@ extern "C" int bfa_append_paged_kv_fp4(const void* k, const void* v, int kv_dtyp
   const hipStream_t s = as_stream(stream);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (vec) hipLaunchKernelGGL((kv_fp4_append_kernel<DT, true>), fp4_grid(f), dim3(256), 0, s, f);
-    else hipLaunchKernelGGL((kv_fp4_append_kernel<DT, false>), fp4_grid(f), dim3(256), 0, s, f);
+    if (!vec) hipLaunchKernelGGL((kv_fp4_append_kernel<DT, false, 1>), fp4_grid(f, 1), dim3(256), 0, s, f);
+    else if (fp4_many(f)) hipLaunchKernelGGL((kv_fp4_append_kernel<DT, true, 4>), fp4_grid(f, 4), dim3(256), 0, s, f);
+    else hipLaunchKernelGGL((kv_fp4_append_kernel<DT, true, 1>), fp4_grid(f, 1), dim3(256), 0, s, f);
   };
   switch (kv_dtype) {
     case BFA_DTYPE_BF16: launch(std::integral_constant<int, BFA_DTYPE_BF16>{}); break;
@@ -232,10 +288,15 @@ extern "C" int bfa_gather_paged_kv_fp4(const void* codes, const void* scales, in
   BFA_REQUIRE(k_out && v_out && aligned16(k_out) && aligned16(v_out), "%s: outputs must be 16-byte aligned", what);
   f.k_out = k_out; f.v_out = v_out;
   const hipStream_t s = as_stream(stream);
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (fp4_many(f)) hipLaunchKernelGGL((kv_fp4_gather_kernel<DT, 4>), fp4_grid(f, 4), dim3(256), 0, s, f);
+    else hipLaunchKernelGGL((kv_fp4_gather_kernel<DT, 1>), fp4_grid(f, 1), dim3(256), 0, s, f);
+  };
   switch (out_dtype) {
-    case BFA_DTYPE_BF16: hipLaunchKernelGGL((kv_fp4_gather_kernel<BFA_DTYPE_BF16>), fp4_grid(f), dim3(256), 0, s, f); break;
-    case BFA_DTYPE_F16: hipLaunchKernelGGL((kv_fp4_gather_kernel<BFA_DTYPE_F16>), fp4_grid(f), dim3(256), 0, s, f); break;
-    default: hipLaunchKernelGGL((kv_fp4_gather_kernel<BFA_DTYPE_F32>), fp4_grid(f), dim3(256), 0, s, f); break;
+    case BFA_DTYPE_BF16: launch(std::integral_constant<int, BFA_DTYPE_BF16>{}); break;
+    case BFA_DTYPE_F16: launch(std::integral_constant<int, BFA_DTYPE_F16>{}); break;
+    default: launch(std::integral_constant<int, BFA_DTYPE_F32>{}); break;
   }
   return check_launch(what);
 }

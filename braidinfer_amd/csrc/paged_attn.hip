@@ -1101,7 +1101,10 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
                             int64_t num_indices, int64_t page_size, int64_t window, int64_t sinks) {
   PagedPlan p{};
   const int64_t rows = tokens * group;
-  p.rb = rows <= 16 * num_seqs ? 0 : rows <= 64 * num_seqs ? 1 : 2;
+  // tiles of 128 rows by 64 keys, over all kv heads, if every request had the average
+  const int64_t keys = cdiv(num_indices * page_size, num_seqs), seen = window > 0 ? std::min(keys, window + sinks + 64) : keys;
+  const int64_t big = (rows / 128 + num_seqs) * hkv * cdiv(seen, 64);
+  p.rb = rows <= 16 * num_seqs || big < 600 ? 0 : rows <= 64 * num_seqs || big < 3000 ? 1 : 2;
   const int forced = tuning(BFA_TUNE_PAGED_ROWS);  // planner override
   if (forced == 16 || forced == 64 || forced == 128) p.rb = forced / 64;
   p.bm = p.rb == 0 ? 16 : 64 * p.rb;
@@ -1109,13 +1112,14 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
   p.shape = paged_shape(p.bm, static_cast<int32_t>(group), static_cast<int32_t>(kt), static_cast<int32_t>(window),
                         static_cast<int32_t>(sinks));
   p.nblocks = static_cast<int32_t>(std::min(rows, rows / p.bm + num_seqs));
-  p.least = p.rb == 0 ? 4 : 2;
+  p.least = p.rb == 0 ? 4 : 8;
   const int64_t all = cdiv(num_indices * page_size, kt) + num_seqs;  // key tiles of all requests
   const int64_t most = std::min<int64_t>(all, p.shape.most);        // of a block
+  const int64_t work = p.rb == 0 ? std::min(all, p.nblocks * most) : p.nblocks * std::min(most, cdiv(all, num_seqs));
+  int64_t wgs = p.rb == 0 ? std::min<int64_t>(std::max<int64_t>(work * hkv / 24, 640), 2048) : 512;
   const int wanted = tuning(BFA_TUNE_PAGED_WG);  // planner override
-  int64_t wish = cdiv(wanted > 0 ? wanted : p.rb == 0 ? 2560 : 512, hkv);
-  if (wanted <= 0) wish = std::max<int64_t>(wish - p.nblocks, cdiv(wish, 4));
-  p.target = static_cast<int32_t>(std::max<int64_t>(1, std::min(wish, std::min(all, p.nblocks * most) / p.least)));
+  if (wanted > 0) wgs = wanted;
+  p.target = static_cast<int32_t>(std::max<int64_t>(1, std::min(cdiv(wgs, hkv), work / p.least)));
   p.split = most > p.least && (p.rb == 0 ? p.nblocks * hkv < 8192 : p.nblocks * hkv < 1024);
   if (wanted >= 0) p.split = wanted > 0 && most > p.least;
   p.items = p.nblocks + (p.split ? p.target : 0);

@@ -13,7 +13,7 @@ from braidinfer_amd import _lib
 from braidinfer_amd.kernels import Fp4KVCache
 from braidinfer_amd.layers import paged_attention
 from tests.helpers import gen
-from tests.paged_reference import attention64, attention_allowance, from_fp4, make_batch, to_fp4
+from tests.paged_reference import attention64, attention_allowance, from_fp4, make_batch, request_rows, to_fp4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -39,6 +39,17 @@ def make_cache(seed, batch, hkv, d, kind, dtype, layout="HND", fill=None):
         return Fp4KVCache(codes.to(DEV), scales.to(DEV)), from_fp4(codes, scales).to(DEV)
     x = x.to(dtype)
     return (x if layout == "HND" else x.transpose(2, 3).contiguous()), x.double()
+
+
+def attention_without(q, values, batch, s, gone):
+    """64-bit attention of request s's rows without the keys `gone`."""
+    n, m, at = batch.seq[s], batch.query[s], int(batch.qo_indptr[s])
+    group = q.shape[1] // values.shape[2]
+    k, v = (x.repeat_interleave(group, 1).permute(1, 0, 2).contiguous() for x in request_rows(values, batch, s))
+    z = torch.matmul(q[at: at + m].double().permute(1, 0, 2).contiguous(), k.transpose(1, 2).contiguous()) * q.shape[2] ** -0.5
+    hidden = torch.arange(n, device=DEV)[None] > torch.arange(n - m, n, device=DEV)[:, None]
+    hidden[:, list(gone)] = True
+    return torch.matmul(torch.softmax(z.masked_fill(hidden, -math.inf), -1), v).permute(1, 0, 2)
 
 
 def lists(batch):
@@ -89,29 +100,42 @@ def test_windows_and_sinks_over_single_tokens(dtype, kind, hq, hkv, d):
         run(hq + window, [1, 40, 64, 300, 901], [1] * 5, hq, hkv, d, dtype=dtype, kind=kind, window=window, sinks=sinks)
 
 
+# rows of a block and workgroups of the key split: the planner's own choice, and every
+# form, whole and split, at sizes where it would not pick it
+FORMS = [(None, None), (16, 200), (64, 0), (64, 200), (128, 0), (128, 200)]
+
+
+@pytest.mark.parametrize("rows,wgs", FORMS)
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
-def test_prompts(dtype, kind, hq, hkv, d):
+def test_prompts(tuning, dtype, kind, hq, hkv, d, rows, wgs):
     """Whole prompts and pieces over a cached context, of odd lengths, in one batch."""
-    run(hq, [77, 1, 300, 130], [77, 1, 60, 129], hq, hkv, d, dtype=dtype, kind=kind)
+    tuning("PAGED_ROWS", rows), tuning("PAGED_WG", wgs)
+    run(hq, [77, 1, 300, 130, 1100], [77, 1, 60, 129, 40], hq, hkv, d, dtype=dtype, kind=kind)
 
 
+@pytest.mark.parametrize("rows,wgs", [(None, None), (64, 0), (128, 0), (128, 300)])
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("hq,hkv,d", [(32, 4, 64), (16, 8, 128), (15, 3, 128)])
-def test_prompts_with_windows(dtype, kind, hq, hkv, d):
+def test_prompts_with_windows(tuning, dtype, kind, hq, hkv, d, rows, wgs):
+    tuning("PAGED_ROWS", rows), tuning("PAGED_WG", wgs)
     for window, sinks in ((1, 0), (17, 1), (64, 64), (65, 4), (200, 130)):
         run(window, [210, 333, 64], [210, 100, 64], hq, hkv, d, dtype=dtype, kind=kind, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("rows", [None, 64, 128])
 @pytest.mark.parametrize("ps", [1, 3, 16, 64, 100])
 @pytest.mark.parametrize("kind", ["16", "fp4"])
-def test_page_sizes(ps, kind):
+def test_page_sizes(tuning, ps, kind, rows):
+    tuning("PAGED_ROWS", rows)
     run(ps, [1, 99, 100, 101, 260], [1] * 5, 8, 2, 64, ps=ps, kind=kind, window=90, sinks=2)
     run(ps, [150, 260], [150, 100], 8, 2, 128, ps=ps, kind=kind)
 
 
+@pytest.mark.parametrize("rows", [None, 128])
 @pytest.mark.parametrize("layout", ["HND", "NHD"])
-def test_layouts(layout):
+def test_layouts(tuning, layout, rows):
+    tuning("PAGED_ROWS", rows)
     run(1, [5, 200, 64], [1, 1, 1], 16, 4, 128, layout=layout)
     run(2, [5, 200, 64], [5, 150, 3], 16, 4, 128, layout=layout, window=70, sinks=4)
 
@@ -138,14 +162,20 @@ def test_many_requests():
     run(10, seq, [min(n, 1 + 31 * (i % 5 == 0)) for i, n in enumerate(seq)], 16, 2, 64)
 
 
+@pytest.mark.parametrize("rows", [16, 64, 128])
 @pytest.mark.parametrize("scale", [1.0, -0.3, 0.0, 1e-3])
-def test_scales(scale):
+def test_scales(tuning, scale, rows):
+    tuning("PAGED_ROWS", rows)
     run(11, [70, 300], [20, 1], 8, 2, 64, scale=scale)
 
 
-def test_scores_that_leave_one_key():
-    """Scores in the thousands, so that a row is all but one key's value."""
-    run(12, [70, 300, 5], [20, 1, 5], 8, 2, 128, std=300.0)
+@pytest.mark.parametrize("rows", [16, 64, 128])
+@pytest.mark.parametrize("std", [300.0, 1e6])
+def test_scores_that_leave_one_key(tuning, std, rows):
+    """Scores in the thousands and in the millions (where the product with the scale is
+    rounded before the difference), so that a row is all but one key's value."""
+    tuning("PAGED_ROWS", rows)
+    run(12, [70, 300, 5], [20, 1, 5], 8, 2, 128, std=std)
 
 
 def test_rows_that_see_nothing():
@@ -182,16 +212,18 @@ def test_rows_behind_the_last_request_stay():
         check(out, q, values, batch, 0.125, None, 0)
 
 
+@pytest.mark.parametrize("rows,ps", [(16, 16), (64, 16), (128, 16), (128, 5)])
 @pytest.mark.parametrize("kind", ["16", "fp4"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_a_key_reaches_only_the_rows_that_see_it(kind, bad):
+def test_a_key_reaches_only_the_rows_that_see_it(tuning, kind, bad, rows, ps):
     """A token whose key and value are not finite, in the middle of a prompt and of a few
     drafted tokens: rows before it, and rows whose window has passed it, are as without."""
     for seq, query, window in (([150], [150], None), ([300], [150], 40), ([300], [4], None), ([300], [4], 2)):
-        batch = make_batch(15, seq, query, 16)
+        tuning("PAGED_ROWS", rows)
+        batch = make_batch(15, seq, query, ps)
         cache, values = make_cache(15, batch, 2, 64, kind, BF16)
         at = seq[0] - query[0] // 2 - 1
-        page, slot = int(batch.kv_indices[at // 16]), at % 16
+        page, slot = int(batch.kv_indices[at // ps]), at % ps
         if kind == "fp4":
             cache.scales[page, 1, :, slot, 1] = 255
             values[page, 1, :, slot, 32:] = math.nan
@@ -200,8 +232,8 @@ def test_a_key_reaches_only_the_rows_that_see_it(kind, bad):
             values[page, 1, :, slot, 5] = bad
         q = torch.randn(query[0], 4, 64, device=DEV).to(BF16)
         got = paged_attention(q, cache, *lists(batch), window=window)
-        rows = torch.arange(query[0]) + seq[0] - query[0]
-        clean = (rows < at) | (rows - at >= (window or 10 ** 9))
+        pos = torch.arange(query[0]) + seq[0] - query[0]
+        clean = (pos < at) | (pos - at >= (window or 10 ** 9))
         assert bool(clean.any()) and torch.isfinite(got[clean]).all()
         assert not torch.isfinite(got[~clean]).all(-1).any()
         want, parts = attention64(q, values, batch, 0.125, window)
@@ -216,8 +248,10 @@ def test_a_key_reaches_only_the_rows_that_see_it(kind, bad):
             assert torch.isfinite(got[clean]).all() and not torch.isfinite(got[~clean]).any()
 
 
-def test_pages_and_offsets_that_do_not_exist():
+@pytest.mark.parametrize("rows", [16, 64, 128])
+def test_pages_and_offsets_that_do_not_exist(tuning, rows):
     """Each is told, and what is there is attended all the same."""
+    tuning("PAGED_ROWS", rows)
     batch = make_batch(16, [40, 70, 33], [1, 30, 1], 16)
     cache, values = make_cache(16, batch, 2, 64, "16", BF16)
     q = torch.randn(32, 4, 64, device=DEV).to(BF16)
@@ -236,9 +270,13 @@ def test_pages_and_offsets_that_do_not_exist():
 
     for page in (batch.num_pages, -batch.num_pages - 1, 2 ** 31 - 1, -2 ** 31):
         bad = idx.clone()
-        bad[4] = page  # the middle of the second request
+        bad[4] = page  # keys 16 .. 31 of the second request
         got = told(idx=bad)
-        assert torch.equal(got[0], good[0]) and torch.equal(got[31], good[31]) and torch.isfinite(got).all()
+        assert torch.equal(got[0], good[0]) and torch.equal(got[31], good[31])
+        # (half a step of the weights and of the result, and as much for scores of up to 128)
+        want = attention_without(q, values, batch, 1, range(16, 32))
+        off = (got[1:31].double().reshape(30, 4, 64) - want).abs()
+        assert float(off.max()) < 3 * 2.0 ** -8 * float(torch.nan_to_num(values).abs().max())
     # (s: as it was, 0: left out, -: more pages than the request has, whose unused slots are NaN)
     for t, kinds in (([0, 3, 8, 99], "ss0"), ([-1, 3, 8, 11], "0ss"), ([0, 9, 8, 11], "-0s"), ([0, 3, 2 ** 31 - 1, 11], "s00")):
         got = told(ptr=torch.tensor(t, dtype=torch.int32, device=DEV))
