@@ -14,6 +14,7 @@
 // for another.  Bound by that latency: two dependent reads and the writes.
 #include "bfa_device.h"
 #include "bfa_host.h"
+#include "bfa_paged_scan.h"
 
 namespace bfa {
 
@@ -58,29 +59,31 @@ __device__ __forceinline__ Lengths request_lengths(const BatchArgs& a, int64_t b
 }
 
 __global__ __launch_bounds__(256) void paged_batch_kernel(BatchArgs a) {
-  __shared__ int64_t part[4][4];
+  __shared__ int32_t part[4][4];
   const int tid = threadIdx.x;
   const int64_t b = blockIdx.x;
-  int64_t sum[4] = {0, 0, 0, 0};  // pages and queries before b, of all
+  // pages and queries before b, and of all, held at 2^30 - 1 (there is room for fewer)
+  int32_t sum[4] = {0, 0, 0, 0};
   for (int64_t c = tid; c < a.num_seqs; c += 256) {
     bool bad;
     const Lengths l = request_lengths(a, c, bad);
-    sum[2] += l.pages;
-    sum[3] += l.query;
+    const int32_t pages = static_cast<int32_t>(min<int64_t>(l.pages, PAGED_MOST));
+    const int32_t query = static_cast<int32_t>(min<int64_t>(l.query, PAGED_MOST));
+    sum[2] = paged_add(sum[2], pages);
+    sum[3] = paged_add(sum[3], query);
     if (c < b) {
-      sum[0] += l.pages;
-      sum[1] += l.query;
+      sum[0] = paged_add(sum[0], pages);
+      sum[1] = paged_add(sum[1], query);
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum[k] += __shfl_xor(sum[k], d);
+    sum[k] = sum_lanes(sum[k]);
     if ((tid & 63) == 0) part[tid >> 6][k] = sum[k];
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 4; ++k) sum[k] = part[0][k] + part[1][k] + part[2][k] + part[3][k];
+  for (int k = 0; k < 4; ++k) sum[k] = paged_add(paged_add(part[0][k], part[1][k]), paged_add(part[2][k], part[3][k]));
   const int64_t page0 = sum[0], token0 = sum[1], all_pages = sum[2], all_tokens = sum[3];
   const int64_t nt = static_cast<int64_t>(gridDim.y) * 256, first = static_cast<int64_t>(blockIdx.y) * 256 + tid;
   if (b < a.num_seqs) {
@@ -142,8 +145,8 @@ extern "C" int bfa_build_paged_kv_batch(const void* page_tables, int page_tables
   const int64_t lim = int64_t{1} << 31;
   BFA_REQUIRE(num_seqs >= 0 && max_pages >= 0 && num_tokens >= 0 && num_indices >= 0 && page_table_stride >= 0, "%s: bad geometry", what);
   BFA_REQUIRE(page_size > 0, "%s: page_size must be positive", what);
-  BFA_REQUIRE(num_seqs < lim / 2 && num_tokens < lim && num_indices < lim && max_pages < lim && page_size < lim,
-              "%s: 2^31 requests, pages or tokens or more", what);
+  BFA_REQUIRE(num_seqs < lim / 2 && num_tokens < lim / 2 && num_indices < lim / 2 && max_pages < lim && page_size < lim,
+              "%s: 2^30 requests, pages or tokens or more", what);
   BFA_REQUIRE(qo_indptr && kv_indptr, "%s: null pointer", what);
   BFA_REQUIRE(num_seqs == 0 || (seq_lens && query_lens && kv_last_page_len && (max_pages == 0 || page_tables)), "%s: null pointer", what);
   BFA_REQUIRE((num_indices == 0 || kv_indices) && (num_tokens == 0 || (batch_indices && positions && slot_mapping)),

@@ -508,7 +508,8 @@ int bfa_linear(const void* x, int dtype, int64_t tokens, int64_t k, int64_t x_st
  * request.  A negative length, a seq_len past the page table, a query_len past the
  * seq_len, and pages or tokens past num_indices / num_tokens set
  * BFA_STATUS_INDEX_OOB: the length is then taken as 0, the pages are those of the
- * table, such tokens have slot -1, and what does not fit is left out. */
+ * table, such tokens have slot -1, and what does not fit is left out.  num_tokens and
+ * num_indices below 2^30. */
 int bfa_build_paged_kv_batch(const void* page_tables, int page_tables_dtype, int64_t num_seqs,
                              int64_t max_pages, int64_t page_table_stride, const void* seq_lens,
                              int seq_lens_dtype, const void* query_lens, int query_lens_dtype,

@@ -201,7 +201,7 @@ def test_batch_entry_refuses():
         return rc("bfa_build_paged_kv_batch", *a.values())
 
     for change, match in ((dict(tdt=_lib.F32), "int32/int64"), (dict(seqs=-1), "geometry"), (dict(ps=0), "page_size"),
-                          (dict(tokens=1 << 31), "2^31 requests"), (dict(seq=None), "null pointer"),
+                          (dict(tokens=1 << 30), "2^30 requests"), (dict(seq=None), "null pointer"),
                           (dict(kv=None), "null pointer"), (dict(slots=None), "null output"), (dict(idx=None), "null output")):
         code, text = batch(**change)
         assert code == -1 and match in text, (change, text)
