@@ -336,14 +336,15 @@ def require_device(*tensors: torch.Tensor | None) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError(
-                "braidinfer_amd ops run only on ROCm devices (got a tensor on "
-                f"{t.device}); there is no CPU path")
-        if first is None:
-            first, idx = t, t.get_device()
-        elif t.get_device() != idx:
-            raise RuntimeError(f"braidinfer_amd: tensors on different devices ({first.device}, {t.device})")
+        i = t.get_device()
+        if i != idx or i < 0:
+            if not t.is_cuda:
+                raise RuntimeError(
+                    "braidinfer_amd ops run only on ROCm devices (got a tensor on "
+                    f"{t.device}); there is no CPU path")
+            if first is not None:
+                raise RuntimeError(f"braidinfer_amd: tensors on different devices ({first.device}, {t.device})")
+            first, idx = t, i
     if first is None:
         raise RuntimeError("braidinfer_amd: no device tensor given")
     return first.device

@@ -411,11 +411,19 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedArgs a) {
     for (int32_t at = blocks + tid; at < a.nblocks; at += 1024) a.table[at] = make_int4(0, 0, 0, 0);
 }
 
+// (in scalar registers: the compiler does not see by itself that a wave's lanes agree,
+// and kept the key loops' counters and branches in vector ones)
 __device__ __forceinline__ Item find_item(const PagedArgs& a, int32_t x, bool writes_table) {
-  if (!a.plan) return locate(a, x, writes_table);
-  const int4 p = a.plan[2 * x], q = a.plan[2 * x + 1];
+  Item it;
+  if (!a.plan) {
+    it = locate(a, x, writes_table);
+  } else {
+    const int4 p = a.plan[2 * x], q = a.plan[2 * x + 1];
+    it = Item{PagedSeq{p.x, p.y, p.z, p.w, q.x}, q.y, q.z, q.w};
+  }
   auto rd = [](int32_t v) { return __builtin_amdgcn_readfirstlane(v); };
-  return Item{PagedSeq{rd(p.x), rd(p.y), rd(p.z), rd(p.w), rd(q.x)}, rd(q.y), rd(q.z), rd(q.w)};
+  return Item{PagedSeq{rd(it.s.q0), rd(it.s.qlen), rd(it.s.page0), rd(it.s.npages), rd(it.s.kvlen)}, rd(it.block), rd(it.chunk),
+              rd(it.chunks)};
 }
 
 // The rows of a block: positions and query addresses.
