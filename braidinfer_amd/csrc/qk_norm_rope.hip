@@ -63,8 +63,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a) {
   const int e = act ? 8 * j : 0;
   const T* x = static_cast<const T*>(a.x[s]) + t * a.st[s] + h * a.sh[s] + e;
   float x1[8], x2[8], c[8], n[8];
-  load8_nt<DT>(x, x1);
-  load8_nt<DT>(x + half, x2);
+  load8<DT>(x, x1);
+  load8<DT>(x + half, x2);
   bool ok;
   const int64_t p = qk_position(a, t, ok);
   if (!ok && j == 0) flag_status(a.status, BFA_STATUS_INDEX_OOB);
