@@ -6,8 +6,9 @@
 // over the keys j that row r sees (bfa_paged.h); a row that sees none is 0.  A row
 // is a query token and one of the Hq / Hkv query heads of a kv head, so a key that
 // is read serves all of them.  Scores, maxima, sums and accumulators are fp32; the
-// weights p are rounded to the queries' 16-bit type for the matrix product (at most
-// half a step, 2^-8 of p in bf16 and 2^-11 in fp16, and the row's largest p is exactly 1).
+// weights p are rounded to the queries' 16-bit type for the matrix product (by at most
+// half a step, 2^-8 of p in bf16 and 2^-11 in fp16), since the matrix cores take V in
+// that type, and the sum below adds them before that; the output is rounded once.
 //
 // The 4-bit cache holds E2M1 codes, two to a byte, and a power-of-two scale (E8M0)
 // for each 32 elements of a row.  v_cvt_scalef32_pk_bf16_fp4 gives two elements'
@@ -185,7 +186,11 @@ __device__ __forceinline__ uint4 v_fragment(const uint4* tile, int key0, int jd,
 // on, where it could carry a weight past the type, the product is rounded first, as m's
 // was.  m follows a larger score only when that is more than LAG above it: weights then
 // reach 2^LAG, which fp32 sums and 16-bit weights do not mind, and most tiles after a
-// row's first few leave the accumulators alone.
+// row's first few leave the accumulators alone.  (Measured, 8192 tokens of 32 heads of
+// 128 over a window of 4096, and 64 requests of up to 8000 tokens in 4 bits: 483 and
+// 78.7 us with LAG 0, 474 and 79.4 with 2, 463 and 76.3 with 6.  A row's largest weight
+// is 1 with LAG 0, which 16 bits hold exactly; with 6 it is rounded as the others are,
+// and the largest error of an output is 1.1 to 1.15 times that of LAG 0.)
 template <bool BF16, int D, int KC, int RB>
 __device__ __forceinline__ void attend(pa_f32x4_t (&sc)[RB][KC], float sl2, float (&m)[RB], float (&l)[RB],
                                        pa_f32x4_t (&o)[RB][D / 16], const uint4* vt, int lane) {
@@ -348,8 +353,10 @@ __device__ __forceinline__ Item locate(const PagedArgs& a, int32_t x, bool write
 }
 
 // The same for more requests, by one workgroup ahead of the others: all items, and the
-// table, 1024 requests at a time.  (512 requests of one key each: the items found by
-// every workgroup for itself TIME_INLINE, so TIME_PLAN.)
+// table, 1024 requests at a time.  (512 requests of one key each: 99 us with the items
+// found by every workgroup for itself, a pass of 64 requests after another, 41 so.  One
+// pass is cheaper than the launch: 64 requests of one key 8.8 us found inline and 13.4
+// planned, one of 4000 keys 12.1 and 16.6, 64 of up to 4000 in a window 181 and 186.)
 __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedArgs a) {
   __shared__ int32_t item_end[1024], block_end[1024], wave_sum[2][16];
   const int tid = threadIdx.x, wid = tid >> 6;
@@ -477,7 +484,10 @@ __device__ __forceinline__ KeyRow key_row(const PagedArgs& a, const PagedSeq& s,
 // multiple of 16 lie on one page, so a lane resolves such a group (lane c group c), and
 // a load's address is the group's, in scalar registers, and an offset that the lane
 // keeps; otherwise a lane resolves a key, and loads take their rows' offsets from it.
-// (The 4-bit decode form is bound by the instructions it issues: TIME_P16.)
+// (It is fewer instructions, 300 in place of 393 on the vector unit per 32 keys of the
+// 4-bit decode form, and lets the prefill form stage by DMA: 8192 tokens of 32 heads of
+// 128 over a window of 4096 567 -> 464 us, 64 requests of up to 4000 keys 182 -> 175,
+// 30 requests of up to 8000 in 4 bits 17.3 -> 15.7.)
 template <bool FP4, bool P16, int KT>
 struct KeyTile {
   KeyRow kr;
@@ -574,8 +584,11 @@ __device__ __forceinline__ void poison(const PagedArgs& a, const PagedSeq& s, in
 // the item by itself, with its own running state, and the four meet in the LDS at
 // the end.  K fragments go from the cache straight to the registers that the
 // product reads; V goes through the wave's own LDS tile, for the transposing reads.
-// The next tile's rows are in flight during a tile's work, and the page ids of the
-// one after.  Bound by the cache's bytes.
+// The page ids of the next tile are asked for during a tile's work; its rows are not
+// (a second tile's registers cost more than they hid: the CU's other waves fill the
+// wait).  Bound by the cache's bytes: 64 requests of 32 heads of 128 on 8,
+// window 4000, 931 MB, in 176 us are 5.3 TB/s, above a large copy's 4.9.  In 4 bits the
+// conversions weigh as much: 64 requests of up to 8000 keys, 281 MB, in 72 us, 3.9 TB/s.
 template <bool BF16, int D, bool FP4, bool P16>
 __global__ __launch_bounds__(256, 3) void paged_decode_kernel(PagedArgs a) {
   constexpr int KT = 32, KC = KT / 16;
@@ -776,9 +789,15 @@ __global__ __launch_bounds__(256, 3) void paged_decode_kernel(PagedArgs a) {
 
 // ----------------------------------------------------------------- prefill
 // Blocks of 64 RB rows, one kv head, 4 waves of 16 RB rows each over the same key
-// tiles of 64, which all of them load into the LDS (two tiles: the next one's rows
-// are in flight in registers during a tile's matrix work).  Bound by the matrix
-// cores and the LDS that feeds them.
+// tiles of 64, which all of them load into the LDS, two tiles deep: the next one's rows
+// are on their way during a tile's matrix work, by DMA where a tile's keys lie on whole
+// 16-key pages of 16-bit elements, in registers otherwise.  RB is 2 where there are rows
+// for it, since a K or V fragment read from the LDS then feeds two products.  Bound by
+// what the waves issue between the products, the softmax above all (85 % of the cycles
+// issue, 37 % of them to the matrix cores, no bank conflicts): 8192 tokens of 32 heads of
+// 128 on 8, window 4096, 413 GFLOP, in 460 us are 897 TFLOP/s; a large bf16 product has
+// 1365.  In 4 bits a tile is converted once a workgroup, on its way to the LDS: 1000
+// tokens of 16 heads on 8 over 9000, 70 GFLOP, in 109 us.
 template <bool BF16, int D, bool FP4, bool P16, int RB>
 __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   constexpr int KT = 64, KC = 4, BM = 64 * RB;
@@ -1011,7 +1030,8 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 // ------------------------------------------------------------------- merge
 // Joins the items of each block that has several: a wave takes a row, or up to 16
 // items of it at a time where there are more and the workgroup's four waves share the
-// row (30000 keys of one request: TIME_MERGE); D / 4 lanes have 4 columns each, the 64 /
+// row (30000 keys of one request, 128 items: attention and join 42.3 us with a wave a
+// row, 35.0 so; 256 items 49 and 38.5); D / 4 lanes have 4 columns each, the 64 /
 // (D / 4) groups of lanes every such item, and meet by lane exchanges, the waves in the
 // LDS, in one order whatever runs first.
 template <bool BF16, int D, int BM>
@@ -1085,8 +1105,8 @@ struct PagedPlan {
   int64_t total() const { return acc_bytes + ml_bytes + table_bytes + plan_bytes; }
 };
 
-// The form follows the rows of an average request, and the items the workgroups that
-// fill the chip; the lengths themselves stay on the device.
+// The form follows the rows of an average request and the whole call's work, and the
+// items the workgroups that fill the chip; the lengths themselves stay on the device.
 static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int64_t hkv, int64_t d,
                             int64_t num_indices, int64_t page_size, int64_t window, int64_t sinks) {
   PagedPlan p{};
@@ -1094,6 +1114,14 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
   // tiles of 128 rows by 64 keys, over all kv heads, if every request had the average
   const int64_t keys = cdiv(num_indices * page_size, num_seqs), seen = window > 0 ? std::min(keys, window + sinks + 64) : keys;
   const int64_t big = (rows / 128 + num_seqs) * hkv * cdiv(seen, 64);
+  // Blocks of 16 rows for requests of as few, and where 128-row blocks would be so few
+  // tiles that the chip is not full; of 128 where the work is ample and rows fill them.
+  // us with blocks of 16 / 64 / 128 (`big`): a prompt of 100, 16 heads on 8 (32)
+  // 9.3 / 9.3 / 11.0; three of 300, window 130 (about 300) 12.8 / 17.9 / 21.8; one of 500, 32 on
+  // 8 (1024) 23.7 / 20.9 / 24.8; four of up to 1000, 16 on 8 (about 2000) 34.4 / 32.8 /
+  // 39.7; one of 2000, 32 on 8 (16128) 165 / 73.4 / 75.8; 500 tokens over 3000, 32 on 4 of
+  // 64 (6016) 59.5 / 46.5 / 43.8; 200 over 6000, 32 on 8 (5264) 111 / 80 / 48.4; 1000 over
+  // 9000 in 4 bits, 16 on 8 (18048) 189 / 152 / 112; 8192 tokens 1763 / 702 / 476.
   p.rb = rows <= 16 * num_seqs || big < 600 ? 0 : rows <= 64 * num_seqs || big < 3000 ? 1 : 2;
   const int forced = tuning(BFA_TUNE_PAGED_ROWS);  // planner override
   if (forced == 16 || forced == 64 || forced == 128) p.rb = forced / 64;
@@ -1102,14 +1130,26 @@ static PagedPlan paged_plan(int64_t tokens, int64_t num_seqs, int64_t group, int
   p.shape = paged_shape(p.bm, static_cast<int32_t>(group), static_cast<int32_t>(kt), static_cast<int32_t>(window),
                         static_cast<int32_t>(sinks));
   p.nblocks = static_cast<int32_t>(std::min(rows, rows / p.bm + num_seqs));
+  // Key tiles of an item at least: one for each wave of the decode form; 8 of the prefill
+  // form, whose split pays for partial sums of 64 rows and more (the prompt of 500 above
+  // in blocks of 64: 20.7 us whole, 28.6 split).
   p.least = p.rb == 0 ? 4 : 8;
   const int64_t all = cdiv(num_indices * page_size, kt) + num_seqs;  // key tiles of all requests
   const int64_t most = std::min<int64_t>(all, p.shape.most);        // of a block
   const int64_t work = p.rb == 0 ? std::min(all, p.nblocks * most) : p.nblocks * std::min(most, cdiv(all, num_seqs));
+  // Workgroups to aim for.  Decode: about 24 tiles (of one kv head) each, from 640, below
+  // which the chip is not full, to 2048, past which partial sums cost more than evenness
+  // gains.  us at 512 / 768 / 1024 / 2048 (work x kv heads): one request of 30000 keys
+  // (7500) 31 / - / 34.6 / 37.8; 8 of up to 4000 in 4 bits 16.0 / 14.9 / 19.4 / -; 64 of up to
+  // 8000 in 4 bits 79.9 / 83.7 / - / 75.8, and 84 at 4096; 64 of up to 16000, window 4000,
+  // - / 187 / - / 177.  Prefill: two a CU, which is what its LDS holds; at 256 / 512 / 768 /
+  // 1024: 1000 tokens over 9000 in 4 bits 170 / 113 / 135 / 121, 200 over 6000 60.6 / 48.7 /
+  // 58.9 / 57.5.
   int64_t wgs = p.rb == 0 ? std::min<int64_t>(std::max<int64_t>(work * hkv / 24, 640), 2048) : 512;
   const int wanted = tuning(BFA_TUNE_PAGED_WG);  // planner override
   if (wanted > 0) wgs = wanted;
   p.target = static_cast<int32_t>(std::max<int64_t>(1, std::min(cdiv(wgs, hkv), work / p.least)));
+  // (blocks that are many times the workgroups the chip holds are even as they are)
   p.split = most > p.least && (p.rb == 0 ? p.nblocks * hkv < 8192 : p.nblocks * hkv < 1024);
   if (wanted >= 0) p.split = wanted > 0 && most > p.least;
   p.items = p.nblocks + (p.split ? p.target : 0);

@@ -2,9 +2,9 @@
 
 A head's row is held in blocks of 32 elements: 32 E2M1 codes (a sign and one of 0, 0.5,
 1, 1.5, 2, 3, 4, 6) and the exponent of the block's power-of-two scale, the smallest
-that keeps the largest magnitude within 6.  An element is off by at most a quarter of
-its block's largest magnitude / 1.5 (half the step between 4 and 6, at a scale just past
-a power of two), and by its block's scale / 4 where it is small.
+that keeps the largest magnitude within 6.  An element is off by at most half a step of
+its magnitude's range: a quarter of the scale up to 2 scales, half of it up to 4, and all
+of it up to 6, which is at most a fifth of the block's largest magnitude.
 
 ``append_paged_kv_fp4`` writes tokens as ``append_paged_kv_batch`` does to a 16-bit
 cache, ``gather_paged_kv_fp4`` reads the stored values back, and
