@@ -141,6 +141,15 @@ BFA_HD int32_t paged_add(int32_t a, int32_t b) {  // of values up to PAGED_MOST
   return a + b > PAGED_MOST ? PAGED_MOST : a + b;
 }
 
+// Whether a block's line of the merge's table, its first item, items, first query row
+// and rows, lies inside what there is.  Every block's does, unless broken offsets, whose
+// requests overlap, make more items than the grid has: then no item may have filled it.
+BFA_HD bool paged_line_inside(int32_t item, int32_t items, int32_t row0, int32_t n, int32_t all_items, int64_t rows,
+                              int32_t bm) {
+  return item >= 0 && items >= 0 && n >= 0 && row0 >= 0 && items <= all_items - item && n <= bm &&
+         static_cast<int64_t>(row0) + n <= rows;
+}
+
 // Key tiles of each of a block's `chunks` items, so that they are alike: with `per`
 // tiles to the first and what is left to the last, the last would often be short.
 BFA_HD int32_t paged_even(int32_t tiles, int32_t chunks) {

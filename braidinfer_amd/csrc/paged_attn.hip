@@ -1042,7 +1042,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const uint32_t block = a.heads.div(blockIdx.x), h = blockIdx.x - block * a.hkv;
   const int4 line = a.table[block];
   const int32_t items = line.y, n = line.w;
-  if (items <= 1) return;
+  if (items <= 1 || !paged_line_inside(line.x, items, line.z, n, a.items, a.tokens * a.group.d, BM)) return;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, sub = lane / L, col = lane % L;
   const bool wide = items > 16;
   const int step_r = (wide ? 1 : 4) * gridDim.y;
@@ -1236,6 +1236,7 @@ extern "C" int bfa_paged_attention(
   const int64_t snk = std::min<int64_t>(sinks, (int64_t{1} << 31) - 1);
   const int64_t group = num_q_heads / num_kv_heads;
   const PagedPlan p = paged_plan(num_tokens, num_seqs, group, num_kv_heads, head_dim, num_indices, page_size, win, snk);
+  BFA_REQUIRE(p.items * num_kv_heads < (int64_t{1} << 24), "%s: too many query rows", what);  // (a launch has 2^32 threads)
   BFA_REQUIRE(p.total() == 0 || (workspace && workspace_bytes >= p.total()), "%s: workspace too small", what);
 
   PagedArgs a{};

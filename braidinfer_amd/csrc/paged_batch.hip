@@ -147,6 +147,7 @@ extern "C" int bfa_build_paged_kv_batch(const void* page_tables, int page_tables
   BFA_REQUIRE(page_size > 0, "%s: page_size must be positive", what);
   BFA_REQUIRE(num_seqs < lim / 2 && num_tokens < lim / 2 && num_indices < lim / 2 && max_pages < lim && page_size < lim,
               "%s: 2^30 requests, pages or tokens or more", what);
+  BFA_REQUIRE(num_seqs < (int64_t{1} << 24), "%s: 2^24 requests or more", what);  // (a launch has 2^32 threads)
   BFA_REQUIRE(qo_indptr && kv_indptr, "%s: null pointer", what);
   BFA_REQUIRE(num_seqs == 0 || (seq_lens && query_lens && kv_last_page_len && (max_pages == 0 || page_tables)), "%s: null pointer", what);
   BFA_REQUIRE((num_indices == 0 || kv_indices) && (num_tokens == 0 || (batch_indices && positions && slot_mapping)),

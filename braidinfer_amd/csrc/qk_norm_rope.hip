@@ -193,6 +193,11 @@ extern "C" int bfa_qk_norm_rope(const void* query, int64_t q_heads, int64_t q_st
   const bool vec = head_dim % 16 == 0 && head_dim <= 1024 && m8(q_stride_token) && m8(q_stride_head) && m8(k_stride_token) &&
                    m8(k_stride_head) && aligned16(query) && aligned16(key) && aligned16(query_out) && aligned16(key_out) &&
                    aligned16(q_norm_weight) && aligned16(k_norm_weight) && aligned16(cos_sin_cache);
+  int64_t lanes = 64;  // of a row
+  if (vec && head_dim <= 256)
+    for (lanes = 2; lanes * 16 < head_dim;) lanes *= 2;
+  BFA_REQUIRE(cdiv(num_tokens * (q_heads + k_heads), 256 / lanes) < (int64_t{1} << 24),  // (a launch has 2^32 threads)
+              "%s: too many rows in one call", what);
   const hipStream_t s = as_stream(stream);
   switch (dtype) {
     case BFA_DTYPE_BF16: launch_qk<BFA_DTYPE_BF16>(a, vec, s); break;

@@ -39,10 +39,13 @@ class Fp4KVCache:
         cs, ss = codes.stride(), scales.stride()
         if (cs[4] != 1 and c[4] > 1) or (ss[4] != 1 and s[4] > 1):
             raise ValueError("codes and scales must have unit stride along head_dim")
-        self.codes, self.scales = codes, scales
-        self.num_pages, _, self.num_kv_heads, self.page_size, half = c
-        self.head_dim = 2 * half
-        self.strides = cs[:4] + ss[:4]  # (page, K|V, head, slot) of the codes and of the scales, in bytes
+        pages, _, heads, slots, half = c
+        strides = cs[:4] + ss[:4]  # (page, K|V, head, slot) of the codes and of the scales, in bytes
+        for name, value in zip(self.__slots__, (codes, scales, pages, heads, slots, 2 * half, strides)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name} of an Fp4KVCache stays as it is: make another of the new tensors")
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device=None) -> "Fp4KVCache":

@@ -69,7 +69,7 @@ def paged_attention(
     code = _QUERY.get(dtype)
     if code is None:
         raise TypeError(f"query must be bf16 or fp16, not {dtype}")
-    if type(kv_cache) is Fp4KVCache:
+    if isinstance(kv_cache, Fp4KVCache):
         if kv_layout != "HND":
             raise ValueError("a 4-bit cache has layout HND")
         data, scales, cache_code, unit = kv_cache.codes, kv_cache.scales, _lib.FP4, 16

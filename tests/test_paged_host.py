@@ -157,6 +157,27 @@ def test_append_and_gather_refuse(change, error, match):
         gather_paged_kv_fp4(a["cache"], a["kv_indices"], None, None, a["positions"], torch.int32)
 
 
+def test_a_cache_keeps_its_tensors():
+    """Calls take the sizes and strides from the time it was made."""
+    cache = Fp4KVCache(torch.zeros(2, 2, 1, 16, 32, dtype=torch.uint8), torch.zeros(2, 2, 1, 16, 2, dtype=torch.uint8))
+    assert (cache.num_pages, cache.num_kv_heads, cache.page_size, cache.head_dim) == (2, 1, 16, 64)
+    with pytest.raises(AttributeError, match="make another"):
+        cache.codes = torch.zeros(1, 2, 1, 16, 32, dtype=torch.uint8)
+
+
+def test_calls_past_a_launch_are_refused():
+    """2^24 workgroups of 256 threads are the 2^32 threads that one launch has at most."""
+    got, text = rc("bfa_paged_attention", *entry_args(tokens=1 << 23, seqs=1 << 23))
+    assert got == -1 and "too many query rows" in text
+    a = dict(q=16, qh=1, qt=64, qs=64, qo=16, k=16, kh=0, kt=0, ks=0, ko=16, dt=_lib.BF16, tokens=1 << 26, d=62, qw=None,
+             kw=None, wdt=0, eps=1e-6, pos=16, pdt=_lib.I64, table=16, most=8, status=None, stream=None)
+    got, text = rc("bfa_qk_norm_rope", *a.values())
+    assert got == -1 and "too many rows" in text
+    got, text = rc("bfa_build_paged_kv_batch", 16, _lib.I32, 1 << 24, 1, 1, 16, _lib.I32, 16, _lib.I32, 16, 1, 1, 16, 16, 16,
+                   16, 16, 16, 16, None, None)
+    assert got == -1 and "2^24 requests" in text
+
+
 def test_fp4_entry_refuses():
     base = (ctypes.c_char * 64)()
     p = (ctypes.addressof(base) + 15) // 16 * 16

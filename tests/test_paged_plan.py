@@ -38,6 +38,9 @@ int even(int tiles, int chunks) { return paged_even(tiles, chunks); }
 int work(int blocks, int tiles, int shift) { return paged_work(PagedSplit{blocks, tiles}, shift); }
 int items(int blocks, int tiles, int per) { return paged_items(PagedSplit{blocks, tiles}, per); }
 int add(int a, int b) { return paged_add(a, b); }
+int line(int item, int items, int row0, int n, int all, long long rows, int bm) {
+  return paged_line_inside(item, items, row0, n, all, rows, bm);
+}
 int per_item(int work, int shift, int target, int least) { return paged_per_item(work, shift, target, least); }
 }
 """
@@ -55,6 +58,7 @@ def lib(tmp_path_factory):
     lib = ctypes.CDLL(str(d / "plan.so"))
     lib.page.restype = ctypes.c_longlong
     lib.page.argtypes = [ctypes.c_longlong] * 2
+    lib.line.argtypes = [ctypes.c_int] * 5 + [ctypes.c_longlong, ctypes.c_int]
     lib.seq.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]
     return lib
 
@@ -164,3 +168,11 @@ def test_sums_of_broken_requests_do_not_overflow(lib):
     assert lib.per_item(most, 0, 1, 2) == most and lib.per_item(most, 20, 1, 2) == most
     assert lib.per_item(0, 0, 300, 4) == 4 and lib.per_item(8192 * 2 ** 16, 10, 320, 4) == most  # (-> 1.7e9 tiles)
     assert lib.per_item(2 ** 20, 10, 320, 4) == -(-2 ** 20 // 320) * 1024
+
+
+def test_lines_of_the_merge_stay_inside(lib):
+    """The table's line of a block that no item filled holds anything."""
+    assert lib.line(0, 4, 0, 16, 4, 16, 16) and lib.line(3, 1, 16, 0, 4, 16, 16)
+    for bad in [(-1, 2, 0, 16), (0, 5, 0, 16), (3, 2, 0, 16), (0, -1, 0, 16), (0, 4, -1, 16), (0, 4, 1, 16), (0, 4, 0, 17),
+                (0, 4, 0, -1), (2**31 - 1, 2**31 - 1, 0, 16), (-2**31, 2, 0, 16), (0, 2, 2**31 - 1, 16)]:
+        assert not lib.line(*bad, 4, 16, 16), bad
