@@ -378,3 +378,23 @@ def test_a_cache_past_four_gigabytes():
     got = paged_attention(q, cache, *lists(batch))
     batch.kv_indices = torch.arange(7, dtype=torch.int32)
     check(got, q, small.double(), batch, d ** -0.5, None, 0)
+
+
+@pytest.mark.parametrize("kind", ["16", "fp4"])
+@pytest.mark.parametrize("rows,wgs", [(16, 0), (16, 300), (64, 0), (64, 300), (128, 300)])
+def test_shared_pages_and_an_output_over_the_queries(tuning, rows, wgs, kind):
+    """Requests that share a prefix list the same pages, one request one page twice; the
+    output may be the queries' own memory, which a block reads before its rows are written."""
+    tuning("PAGED_ROWS", rows), tuning("PAGED_WG", wgs)
+    batch = make_batch(21, [900, 700, 900, 64], [70, 1, 130, 40], 16)
+    at = batch.kv_indptr.tolist()
+    batch.kv_indices[at[1]: at[1] + 40] = batch.kv_indices[:40]
+    batch.kv_indices[at[2]: at[2] + 40] = batch.kv_indices[:40]
+    batch.kv_indices[at[3] + 1] = batch.kv_indices[at[3]]
+    cache, values = make_cache(21, batch, 2, 64, kind, BF16)
+    q = torch.randn(batch.tokens, 8, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(22)).to(BF16)
+    both = q.clone()
+    out = both.view(batch.tokens, 512)
+    assert paged_attention(both, cache, *lists(batch), window=500, num_sinks=3, out=out) is out
+    check(out, q, values, batch, 0.125, 500, 3)
+    braidinfer_amd.check_device_status()
