@@ -797,7 +797,7 @@ __global__ __launch_bounds__(256, 3) void paged_decode_kernel(PagedArgs a) {
 // issue, 37 % of them to the matrix cores, no bank conflicts): 8192 tokens of 32 heads of
 // 128 on 8, window 4096, 413 GFLOP, in 460 us are 897 TFLOP/s; a large bf16 product has
 // 1365.  In 4 bits a tile is converted once a workgroup, on its way to the LDS: 1000
-// tokens of 16 heads on 8 over 9000, 70 GFLOP, in 109 us.
+// tokens of 16 heads on 8 over 9000, 70 GFLOP, in 105 us with the join.
 template <bool BF16, int D, bool FP4, bool P16, int RB>
 __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
   constexpr int KT = 64, KC = 4, BM = 64 * RB;
@@ -1036,7 +1036,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PagedArgs a) {
 // LDS, in one order whatever runs first.
 template <bool BF16, int D, int BM>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  constexpr int L = D / 4, NG = 64 / L, U = 16 / NG;
+  constexpr int L = D / 4, NG = 64 / L;
   __shared__ float4 wacc[4][L];
   __shared__ float wsum[4];
   const uint32_t block = a.heads.div(blockIdx.x), h = blockIdx.x - block * a.hkv;
@@ -1055,7 +1055,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
     const float ref = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
     float4 acc = {};
-    for (int z0 = wide ? 16 * wid : 0; z0 < items; z0 += wide ? 64 : 16) {
+    auto add = [&](int z0, auto n) {  // the items from z0, n at most
+      constexpr int U = decltype(n)::value / NG;
       float2 st[U];
       float4 v[U];
 #pragma unroll
@@ -1071,7 +1072,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
         sum += f * st[u].y;
         acc.x += f * v[u].x; acc.y += f * v[u].y; acc.z += f * v[u].z; acc.w += f * v[u].w;
       }
-    }
+    };
+    // (1000 tokens over 9000 in 4 bits, four items a block: 116.7 us with loads for 16, most
+    // of them again for the last item, and 110.4 so)
+    if (items <= 4) add(0, std::integral_constant<int, 4>{});
+    else for (int z0 = wide ? 16 * wid : 0; z0 < items; z0 += wide ? 64 : 16) add(z0, std::integral_constant<int, 16>{});
 #pragma unroll
     for (int d = L; d < 64; d *= 2) {
       sum += __shfl_xor(sum, d);
@@ -1281,15 +1286,19 @@ extern "C" int bfa_paged_attention(
     constexpr bool B = decltype(bf)::value, F = decltype(four)::value, P = decltype(by16)::value;
     constexpr int DD = decltype(dd)::value;
     const unsigned blocks = static_cast<unsigned>(p.nblocks * num_kv_heads);
+    // Workgroups of the merge over a block's rows, up to one for the four of a pass.  us of
+    // attention and join with 8 / 32: 200 tokens over 6000, 56 blocks of 128 rows, 48.7 /
+    // 46.1; 1000 over 9000 in 4 bits, 128 blocks, 110.4 / 112.3.
+    const unsigned over = std::min(std::max(2048 / blocks, 8u), static_cast<unsigned>(p.bm / 4));
     if (p.rb == 0) {
       hipLaunchKernelGGL((paged_decode_kernel<B, DD, F, P>), grid, dim3(256), 0, s, a);
       if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 16>), dim3(blocks, blocks < 512 ? 4 : 1), dim3(256), 0, s, a);
     } else if (p.rb == 1) {
       hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, P, 1>), grid, dim3(256), 0, s, a);
-      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 64>), dim3(blocks, 4), dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 64>), dim3(blocks, over), dim3(256), 0, s, a);
     } else {
       hipLaunchKernelGGL((paged_prefill_kernel<B, DD, F, P, 2>), grid, dim3(256), 0, s, a);
-      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 128>), dim3(blocks, 8), dim3(256), 0, s, a);
+      if (p.split) hipLaunchKernelGGL((paged_merge_kernel<B, DD, 128>), dim3(blocks, over), dim3(256), 0, s, a);
     }
   };
   auto with_d = [&](auto bf, auto four) {
