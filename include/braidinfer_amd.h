@@ -508,8 +508,8 @@ int bfa_linear(const void* x, int dtype, int64_t tokens, int64_t k, int64_t x_st
  * request.  A negative length, a seq_len past the page table, a query_len past the
  * seq_len, and pages or tokens past num_indices / num_tokens set
  * BFA_STATUS_INDEX_OOB: the length is then taken as 0, the pages are those of the
- * table, such tokens have slot -1, and what does not fit is left out.  num_tokens and
- * num_indices below 2^30. */
+ * table, such tokens have slot -1, and what does not fit is left out.  num_seqs below
+ * 2^24, num_tokens and num_indices below 2^30. */
 int bfa_build_paged_kv_batch(const void* page_tables, int page_tables_dtype, int64_t num_seqs,
                              int64_t max_pages, int64_t page_table_stride, const void* seq_lens,
                              int seq_lens_dtype, const void* query_lens, int query_lens_dtype,
@@ -591,7 +591,8 @@ int bfa_gather_paged_kv_fp4(const void* codes, const void* scales, int64_t num_p
  * bfa_append_paged_kv; a page that does not exist, and offsets outside the arrays,
  * set BFA_STATUS_INDEX_OOB (the page's keys, the request's rows or keys are left
  * out).  out [num_tokens, Hq * head_dim], queries' dtype.  num_indices * page_size
- * and Hq / Hkv * num_tokens below 2^31 and 2^30.  workspace:
+ * and Hq / Hkv * num_tokens below 2^31 and 2^30, and, over all kv heads, fewer than
+ * 2^24 blocks of rows and parts of them; a cache within 64 GiB.  workspace:
  * bfa_paged_attention_workspace_size bytes, 16-byte aligned. */
 int64_t bfa_paged_attention_workspace_size(int64_t tokens, int64_t num_seqs, int64_t num_q_heads,
                                            int64_t num_kv_heads, int64_t head_dim,
