@@ -6,7 +6,9 @@ Drop-in modules mirror the reference package layout:
                                                     apply_rotary_emb, SiluAndMul,
                                                     VocabParallelEmbedding)
 plus rerotate_paged_k (one launch for the cascade differential-RoPE loop) and
-the fused Qwen3 / Llama attention-input chains.  Everything runs through the
+the fused Qwen3 / Llama attention-input chains, and the attention side of a batched
+serving step: build_paged_kv_batch, qk_norm_rope, append_paged_kv_fp4 and
+paged_attention over a 16-bit or a 4-bit paged cache.  Everything runs through the
 C-ABI library braidinfer_amd/lib/libbraidinfer_amd.so; there is no fallback.
 """
 from ._lib import LIB_PATH, BraidinferAMDError, check_device_status, load
